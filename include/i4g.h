@@ -43,7 +43,7 @@ typedef enum {
   I4G_ERR_DRIVER = -6,         /* tensor-map encoding failed */
   I4G_ERR_DEVICE = -7,         /* current device is not sm_100 */
   I4G_ERR_TIMEOUT = -8,        /* a device-side wait hit its limit */
-  I4G_ERR_VARIANT = -9         /* unknown kernel variant */
+  I4G_ERR_VARIANT = -9         /* unknown kernel variant (or activation, scoring) */
 } i4g_status;
 
 /* Kernel selection for i4g_gemm_variant. */
@@ -200,6 +200,107 @@ int i4g_gemm_fp32_ws(const void* A, const uint8_t* tiles, const void* scales,
 int i4g_gemm_static_scratch(const void* A, const uint8_t* tiles,
                             const void* scales, void* C, int M, int N, int K,
                             int group, void* stream);
+
+/* ---- GEMM with a fused epilogue (no counterpart in the reference) ---------- */
+
+/* What happens to each FP32 sum x of the product before the one rounding to C:
+ *   y = act(x + bias)                         C has N columns, or, gated,
+ *   y = act(g + bias_g) * (u + bias_u)        C has N / 2 columns;
+ *   C = y + residual.
+ * Gated weights hold their columns in groups of 16, eight gates and then the
+ * eight columns they gate: output column 8 j + i is made of weight columns
+ * 16 j + i (gate) and 16 j + 8 + i. Activations: SILU x / (1 + exp(-x)),
+ * GELU 0.5 x (1 + erf(x / sqrt 2)), GELU_TANH its tanh approximation. */
+typedef enum {
+  I4G_ACT_NONE = 0,
+  I4G_ACT_RELU = 1,
+  I4G_ACT_SILU = 2,
+  I4G_ACT_GELU = 3,
+  I4G_ACT_GELU_TANH = 4
+} i4g_activation;
+
+typedef struct {
+  const void* bias;      /* fp16 [N], at the weight's columns (per expert:
+                            [E][N]), or NULL */
+  const void* residual;  /* fp16 [M][ld_residual] at C's columns, or NULL; may
+                            be C itself */
+  int ld_residual;       /* row stride of residual, >= C's columns */
+  int activation;        /* i4g_activation */
+  int gated;             /* 0 or 1 */
+  int fp32_out;          /* 0: C is fp16, 1: C is float */
+} i4g_epilogue_t;
+
+/* C = epilogue(A x dequant(B)); A, tiles, scales as for i4g_gemm; C row-major
+ * and contiguous. epilogue NULL: no bias, activation or residual, fp16 C.
+ * M = 0 returns at once. workspace (i4g_gemm_epilogue_workspace_size bytes,
+ * 256-byte aligned, ZEROED ONCE, one per stream, as for i4g_gemm_ws) lets the
+ * tiles of the last, partial wave be cut along K; NULL or too small: whole
+ * tiles. Sums run in a fixed order: results are bitwise reproducible. */
+int i4g_gemm_epilogue_workspace_size(int M, int N, int K, size_t* bytes);
+int i4g_gemm_epilogue(const void* A, const uint8_t* tiles, const void* scales, void* C,
+                      int M, int N, int K, int group, const i4g_epilogue_t* epilogue,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- mixture of experts (no counterpart in the reference) ------------------ */
+
+/* Routing: T tokens' logits [T][ld_logits] (float, or fp16 with
+ * fp32_logits = 0) over E experts -> each token's top_k experts.
+ *   p = softmax or sigmoid of the logits; choice score c = p + bias.
+ *   n_group > 1: experts form n_group runs of E / n_group; a group's score is
+ *     its largest c, or (I4G_GROUP_TOP2) the sum of its two largest; only the
+ *     topk_group best groups' experts can be chosen.
+ *   ids [T][top_k]: the experts of the largest c, best first (ties: lowest
+ *     index); weights [T][top_k]: their p (not c), divided by their sum if
+ *     renormalize, times scale.
+ * A logit of -infinity or NaN, or a bias of -infinity or NaN, takes an expert
+ * out. Where a token has no expert left for a place: id -1, weight 0. The
+ * order of the scores is decided as in FP64.
+ * And the chosen (token, place) pairs in expert order, by token within one
+ * expert (pair = token * top_k + place): offsets [E + 1], expert e has sorted
+ * rows offsets[e] .. offsets[e + 1] - 1; rows [T * top_k], the pair of each
+ * sorted row (-1 past offsets[E]); slots [T][top_k], the sorted row of each
+ * pair (-1 for an id of -1).
+ * E <= 512, top_k <= 32, n_group <= 32; all buffers 4-byte aligned.
+ * workspace: i4g_route_workspace_size bytes (may be 0), 16-byte aligned, one
+ * per stream; it needs no zeroing. T = 0 writes the offsets only. */
+enum { I4G_SCORE_SOFTMAX = 0, I4G_SCORE_SIGMOID = 1 };
+enum { I4G_GROUP_MAX = 0, I4G_GROUP_TOP2 = 1 };
+typedef struct {
+  int scoring;      /* I4G_SCORE_* */
+  int n_group;      /* 1: no groups */
+  int topk_group;   /* groups that stay, 1 .. n_group */
+  int group_score;  /* I4G_GROUP_* */
+  int renormalize;  /* 0 or 1 */
+  float scale;
+} i4g_route_t;
+int i4g_route_workspace_size(int T, int E, size_t* bytes);
+int i4g_route(const void* logits, int fp32_logits, int ld_logits, const float* bias, int T, int E,
+              int top_k, const i4g_route_t* options, int32_t* ids, float* weights,
+              int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace,
+              size_t workspace_bytes, void* stream);
+
+/* The experts' products: row p of C = epilogue(A[src(p)] x dequant(B_e)) for
+ * offsets[e] <= p < offsets[e + 1], with src(p) = rows[p] / row_div (gathered:
+ * row_div = top_k for the tokens' rows) or, rows NULL, p (rows already in
+ * expert order). A has a_rows rows. tiles and scales: the E experts' buffers
+ * one after another. C and the sorted rows have `pairs` rows; those past
+ * offsets[E] are left as they were. The epilogue has no residual (it belongs
+ * to i4g_experts_combine). offsets and rows are read on the device; offsets
+ * outside [0, pairs] are clamped, rows outside A read as zeros. E <= 512.
+ * workspace: as for i4g_gemm_epilogue. pairs = 0 returns at once. */
+int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes);
+int i4g_experts_gemm(const void* A, int a_rows, const uint8_t* tiles, const void* scales, void* C,
+                     const int32_t* offsets, const int32_t* rows, int row_div, int pairs, int E,
+                     int N, int K, int group, const i4g_epilogue_t* epilogue, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* out[t] = residual[t] + sum over places s of weights[t][s] * y[slots[t][s]]
+ * (FP32, in the order of the places, then the residual, one rounding), y fp16
+ * [y_rows][N], residual fp16 [T][N] or NULL (may be out), out fp16 [T][N].
+ * Slots outside [0, y_rows) are skipped. N % 8 == 0, buffers 16-byte aligned.
+ * T = 0 returns at once. */
+int i4g_experts_combine(const void* y, int y_rows, const int32_t* slots, const float* weights,
+                        const void* residual, void* out, int T, int top_k, int N, void* stream);
 
 /* ---- GEMM with the all-gather fused in (no counterpart in the reference) -- */
 

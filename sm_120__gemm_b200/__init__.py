@@ -30,7 +30,11 @@ __all__ = [
     "launch_final_to_peers", "ipc_handle", "ipc_open", "ipc_close", "peer_barrier",
     "shard_range", "device_status", "selftest_wait_timeout", "plan", "set_decode_schedule",
     "kernel_config", "kernel_resources", "max_pairs",
-    "QuantizedLinear", "VARIANT_AUTO", "VARIANT_TC", "VARIANT_DECODE", "DECODE_SCHEDULES",
+    "launch_final_epilogue", "gemm_epilogue_workspace_size", "launch_route",
+    "route_workspace_size", "launch_experts", "experts_workspace_size", "launch_combine",
+    "ACTIVATIONS", "SCORINGS", "GROUP_SCORES", "Epilogue", "RouteOptions",
+    "QuantizedLinear", "QuantizedExperts", "ExpertMLP", "Routing", "route", "combine",
+    "VARIANT_AUTO", "VARIANT_TC", "VARIANT_DECODE", "DECODE_SCHEDULES",
     "PLAN_KERNELS", "PLAN_SCHEDULES", "LIB_PATH",
 ]
 
@@ -86,6 +90,39 @@ _SIGNATURES = {
                          _vp],
     "i4g_layout_version": [],
 }
+
+
+# i4g_activation, I4G_SCORE_*, I4G_GROUP_*
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+class Epilogue(ctypes.Structure):
+    """i4g_epilogue_t."""
+    _fields_ = [("bias", _vp), ("residual", _vp), ("ld_residual", _i), ("activation", _i),
+                ("gated", _i), ("fp32_out", _i)]
+
+
+class RouteOptions(ctypes.Structure):
+    """i4g_route_t."""
+    _fields_ = [("scoring", _i), ("n_group", _i), ("topk_group", _i), ("group_score", _i),
+                ("renormalize", _i), ("scale", ctypes.c_float)]
+
+
+_sz = ctypes.c_size_t
+_SIGNATURES.update({
+    "i4g_gemm_epilogue_workspace_size": [_i, _i, _i, ctypes.POINTER(_sz)],
+    "i4g_gemm_epilogue": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(Epilogue), _vp, _sz,
+                          _vp],
+    "i4g_route_workspace_size": [_i, _i, ctypes.POINTER(_sz)],
+    "i4g_route": [_vp, _i, _i, _vp, _i, _i, _i, ctypes.POINTER(RouteOptions), _vp, _vp, _vp, _vp,
+                  _vp, _vp, _sz, _vp],
+    "i4g_experts_workspace_size": [_i, _i, _i, _i, ctypes.POINTER(_sz)],
+    "i4g_experts_gemm": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
+                         ctypes.POINTER(Epilogue), _vp, _sz, _vp],
+    "i4g_experts_combine": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
+})
 
 
 class _KernelConfig(ctypes.Structure):
@@ -290,6 +327,77 @@ def launch_final_to_peers(a, b_repacked, scales_repacked, dsts, ldc: int, col0: 
           _stream(stream))
 
 
+# ------------------------------------------- fused epilogue, routing, experts
+
+def _size(name: str, *args) -> int:
+    b = _sz()
+    _call(name, *args, ctypes.byref(b))
+    return b.value
+
+
+def _bytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def gemm_epilogue_workspace_size(M: int, N: int, K: int) -> int:
+    """Bytes of zeroed workspace launch_final_epilogue can use for this shape."""
+    return _size("i4g_gemm_epilogue_workspace_size", M, N, K)
+
+
+def experts_workspace_size(pairs: int, E: int, N: int, K: int) -> int:
+    """Bytes of zeroed workspace launch_experts can use for this shape."""
+    return _size("i4g_experts_workspace_size", pairs, E, N, K)
+
+
+def route_workspace_size(T: int, E: int) -> int:
+    """Bytes of workspace launch_route needs (0: none)."""
+    return _size("i4g_route_workspace_size", T, E)
+
+
+def _epilogue(bias, activation: str, gated: bool, residual, ld_residual: int,
+              fp32_out: bool) -> Epilogue:
+    return Epilogue(_ptr(bias), _ptr(residual), ld_residual, ACTIVATIONS[activation], bool(gated),
+                    bool(fp32_out))
+
+
+def launch_final_epilogue(a, b_repacked, scales_repacked, c, M: int, N: int, K: int, group: int,
+                          bias=None, activation: str = "none", gated: bool = False,
+                          residual=None, ld_residual: int = 0, fp32_out: bool = False,
+                          workspace=None, stream=None) -> None:
+    """C ABI i4g_gemm_epilogue: C = act(A x dequant(B) + bias) + residual, or
+    with gated weight columns act(gate) * up; one rounding, at the store."""
+    e = _epilogue(bias, activation, gated, residual, ld_residual, fp32_out)
+    _call("i4g_gemm_epilogue", _ptr(a), _ptr(b_repacked), _ptr(scales_repacked), _ptr(c), M, N, K,
+          group, ctypes.byref(e), _ptr(workspace), _bytes(workspace), _stream(stream))
+
+
+def launch_route(logits, fp32_logits: bool, ld_logits: int, bias, T: int, E: int, top_k: int,
+                 options: RouteOptions, ids, weights, offsets, rows, slots, workspace=None,
+                 stream=None) -> None:
+    """C ABI i4g_route: tokens' experts, weights, and the pairs in expert order."""
+    _call("i4g_route", _ptr(logits), int(fp32_logits), ld_logits, _ptr(bias), T, E, top_k,
+          ctypes.byref(options), _ptr(ids), _ptr(weights), _ptr(offsets), _ptr(rows),
+          _ptr(slots), _ptr(workspace), _bytes(workspace), _stream(stream))
+
+
+def launch_experts(a, a_rows: int, b_repacked, scales_repacked, c, offsets, rows, row_div: int,
+                   pairs: int, E: int, N: int, K: int, group: int, bias=None,
+                   activation: str = "none", gated: bool = False, fp32_out: bool = False,
+                   workspace=None, stream=None) -> None:
+    """C ABI i4g_experts_gemm: the sorted rows' products with their experts' weights."""
+    e = _epilogue(bias, activation, gated, None, 0, fp32_out)
+    _call("i4g_experts_gemm", _ptr(a), a_rows, _ptr(b_repacked), _ptr(scales_repacked), _ptr(c),
+          _ptr(offsets), _ptr(rows), row_div, pairs, E, N, K, group, ctypes.byref(e),
+          _ptr(workspace), _bytes(workspace), _stream(stream))
+
+
+def launch_combine(y, y_rows: int, slots, weights, residual, out, T: int, top_k: int, N: int,
+                   stream=None) -> None:
+    """C ABI i4g_experts_combine: out[t] = residual[t] + sum_s w[t, s] y[slots[t, s]]."""
+    _call("i4g_experts_combine", _ptr(y), y_rows, _ptr(slots), _ptr(weights), _ptr(residual),
+          _ptr(out), T, top_k, N, _stream(stream))
+
+
 def ipc_handle(t) -> tuple[bytes, int]:
     """(64-byte CUDA IPC handle of the allocation holding tensor `t`, byte
     offset of t in it)."""
@@ -392,3 +500,4 @@ def set_decode_schedule(schedule: str) -> None:
 
 
 from .linear import QuantizedLinear  # noqa: E402  (needs the launchers above)
+from .experts import ExpertMLP, QuantizedExperts, Routing, combine, route  # noqa: E402

@@ -1,8 +1,10 @@
 // The C ABI of include/i4g.h: argument checks, device checks, tensor maps
 // and dispatch to the kernels. Nothing here allocates device memory.
 #include "../../include/i4g.h"
+#include "gemm_epi.h"
 #include "gemm_tc.h"
 #include "ptx.cuh"
+#include "route.h"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -301,6 +303,108 @@ int gemm_common(const void* A, const uint8_t* tiles, const void* scales, const i
                                 plan.workspace_bytes > 0 ? workspace : nullptr,
                                 dev->status_word, g_wait_limit_ns, s),
                 "tcgen05 kernel launch");
+}
+
+// Activation map of the epilogue / experts kernel: A [rows][K] fp16, 128-byte
+// swizzle, box 64 (K) x box_rows (1 for the row gather), zeros outside.
+int epi_map(const void* A, int rows, int K, int box_rows, CUtensorMap* map) {
+  EncodeTiledFn encode = nullptr;
+  const int st = encode_fn(&encode);
+  if (st != I4G_OK) return st;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(A), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS
+             ? I4G_OK
+             : fail(I4G_ERR_DRIVER, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
+}
+
+int check_epilogue(const i4g_epilogue_t& e, int N) {
+  if (e.activation < I4G_ACT_NONE || e.activation > I4G_ACT_GELU_TANH)
+    return fail(I4G_ERR_VARIANT, "unknown activation %d", e.activation);
+  if ((e.gated != 0 && e.gated != 1) || (e.fp32_out != 0 && e.fp32_out != 1))
+    return fail(I4G_ERR_VARIANT, "gated (%d) and fp32_out (%d) are 0 or 1", e.gated, e.fp32_out);
+  if (e.residual && e.ld_residual < (e.gated ? N / 2 : N))
+    return fail(I4G_ERR_SHAPE, "ld_residual %d is less than C's %d columns", e.ld_residual,
+                e.gated ? N / 2 : N);
+  if (!aligned(e.bias, 2) || !aligned(e.residual, 2))
+    return fail(I4G_ERR_ALIGNMENT, "bias and residual must be 2-byte aligned");
+  return I4G_OK;
+}
+
+// Rows per weight that choose the tile height of an experts' product: the
+// mean over the experts that can have any.
+int mean_rows(int pairs, int E) { return (pairs + (pairs < E ? pairs : E) - 1) / (pairs < E ? pairs : E); }
+
+// The checks and the launch that i4g_gemm_epilogue (offsets null) and
+// i4g_experts_gemm share; pointers are checked by the caller.
+int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scales, void* C,
+               const int* offsets, const int* rows, int row_div, int M, int E, int N, int K,
+               int group, const i4g_epilogue_t* epilogue, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  const i4g_epilogue_t plain{};
+  const i4g_epilogue_t& e = epilogue ? *epilogue : plain;
+  int st = check_group(K, group, true);
+  if (st != I4G_OK) return st;
+  if ((st = check_epilogue(e, N)) != I4G_OK) return st;
+  if (!aligned(A, 16) || !aligned(tiles, 16) || !aligned(scales, 16))
+    return fail(I4G_ERR_ALIGNMENT, "A, tiles and scales must be 16-byte aligned");
+  if (!aligned(C, e.fp32_out ? 4 : 2))
+    return fail(I4G_ERR_ALIGNMENT, "C must be aligned to its element size");
+  if (!aligned(offsets, 4) || !aligned(rows, 4))
+    return fail(I4G_ERR_ALIGNMENT, "offsets and rows must be 4-byte aligned");
+  if (workspace && !aligned(workspace, 256))
+    return fail(I4G_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != I4G_OK) return st;
+  const int tile_m = i4g::epi::choose_tile(offsets ? mean_rows(M, E) : M);
+  const long tiles_most = i4g::epi::tiles_bound(tile_m, M, E, N);
+  const size_t need = i4g::epi::workspace_bytes(tile_m, tiles_most, K, dev->sm_count);
+  const bool split = workspace && need > 0 && workspace_bytes >= need;
+  CUtensorMap map;
+  if ((st = epi_map(A, a_rows, K, rows ? 1 : tile_m, &map)) != I4G_OK) return st;
+  i4g::epi::Args args{};
+  args.tiles = tiles;
+  args.scales = static_cast<const __half*>(scales);
+  args.C = C;
+  args.offsets = offsets;
+  args.rows = rows;
+  args.row_div = row_div;
+  args.E = E;
+  args.M = M;
+  args.N = N;
+  args.K = K;
+  args.fp32_out = e.fp32_out;
+  args.epilogue = i4g::Epilogue{static_cast<const __half*>(e.bias),
+                                static_cast<const __half*>(e.residual), e.ld_residual,
+                                e.activation};
+  if (split) {
+    args.tickets = static_cast<uint32_t*>(workspace);
+    args.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + i4g::tc::kTicketBytes);
+  }
+  args.status = dev->status_word;
+  args.wait_limit_ns = g_wait_limit_ns;
+  const int grid = i4g::epi::grid_for(tile_m, tiles_most, K, dev->sm_count, split);
+  return finish(i4g::epi::launch(map, tile_m, e.gated != 0, group, args, grid,
+                                 static_cast<cudaStream_t>(stream)),
+                "epilogue GEMM launch");
+}
+
+int check_experts(int pairs, int E, int N, int K) {
+  if (E < 1 || E > i4g::epi::kMaxExperts)
+    return fail(I4G_ERR_SHAPE, "between 1 and %d experts (got %d)", i4g::epi::kMaxExperts, E);
+  if (pairs < 0) return fail(I4G_ERR_SHAPE, "pairs %d is negative", pairs);
+  const int st = check_shape(pairs > 0 ? pairs : 1, N, K);
+  if (st != I4G_OK) return st;
+  // tile indices are 32 bits
+  if (i4g::epi::tiles_bound(16, pairs, E, N) >= (1ll << 30))
+    return fail(I4G_ERR_SHAPE, "pairs=%d N=%d E=%d too large", pairs, N, E);
+  return I4G_OK;
 }
 
 // A kernel that waits on an mbarrier nothing will complete, through the same
@@ -631,6 +735,156 @@ int i4g_gemm_to_peers(const void* A, const uint8_t* tiles, const void* scales, v
   out.col0 = col0;
   return gemm_common(A, tiles, scales, out, false, M, N, K, group, I4G_VARIANT_AUTO, workspace,
                      workspace_bytes, stream);
+}
+
+int i4g_gemm_epilogue_workspace_size(int M, int N, int K, size_t* bytes) {
+  if (!bytes) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  *bytes = 0;
+  int st = check_experts(M, 1, N, K);
+  if (st != I4G_OK) return st;
+  if (M == 0) return I4G_OK;
+  DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != I4G_OK) return st;
+  const int tile_m = i4g::epi::choose_tile(M);
+  *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, M, 1, N), K,
+                                     dev->sm_count);
+  return I4G_OK;
+}
+
+int i4g_gemm_epilogue(const void* A, const uint8_t* tiles, const void* scales, void* C, int M,
+                      int N, int K, int group, const i4g_epilogue_t* epilogue, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const int st = check_experts(M, 1, N, K);
+  if (st != I4G_OK) return st;
+  if (M == 0) return I4G_OK;
+  if (!A || !tiles || !scales || !C) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  return epi_common(A, M, tiles, scales, C, nullptr, nullptr, 1, M, 1, N, K, group, epilogue,
+                    workspace, workspace_bytes, stream);
+}
+
+int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes) {
+  if (!bytes) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  *bytes = 0;
+  int st = check_experts(pairs, E, N, K);
+  if (st != I4G_OK) return st;
+  if (pairs == 0) return I4G_OK;
+  DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != I4G_OK) return st;
+  const int tile_m = i4g::epi::choose_tile(mean_rows(pairs, E));
+  *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, pairs, E, N), K,
+                                     dev->sm_count);
+  return I4G_OK;
+}
+
+int i4g_experts_gemm(const void* A, int a_rows, const uint8_t* tiles, const void* scales, void* C,
+                     const int32_t* offsets, const int32_t* rows, int row_div, int pairs, int E,
+                     int N, int K, int group, const i4g_epilogue_t* epilogue, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  const int st = check_experts(pairs, E, N, K);
+  if (st != I4G_OK) return st;
+  if (epilogue && epilogue->residual)
+    return fail(I4G_ERR_VARIANT, "the experts' product takes no residual");
+  if (pairs == 0) return I4G_OK;
+  if (!A || !tiles || !scales || !C || !offsets)
+    return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  if (rows ? (a_rows < 1 || row_div < 1) : a_rows < pairs)
+    return fail(I4G_ERR_SHAPE, "a_rows=%d row_div=%d for %d pairs", a_rows, row_div, pairs);
+  return epi_common(A, a_rows, tiles, scales, C, offsets, rows, row_div, pairs, E, N, K, group,
+                    epilogue, workspace, workspace_bytes, stream);
+}
+
+static int check_route(int T, int E, int top_k) {
+  if (T < 0 || E < 1 || E > i4g::route::kMaxExperts || top_k < 1 ||
+      top_k > i4g::route::kMaxTopK || top_k > E)
+    return fail(I4G_ERR_SHAPE, "routing T=%d E=%d top_k=%d: E <= 512, top_k <= min(32, E)", T, E,
+                top_k);
+  if (static_cast<long long>(T) * top_k >= (1ll << 31))
+    return fail(I4G_ERR_SHAPE, "routing T=%d top_k=%d too large", T, top_k);
+  return I4G_OK;
+}
+
+int i4g_route_workspace_size(int T, int E, size_t* bytes) {
+  if (!bytes) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  *bytes = 0;
+  int st = check_route(T, E, 1);
+  if (st != I4G_OK) return st;
+  DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != I4G_OK) return st;
+  *bytes = i4g::route::workspace_bytes(T, E, dev->sm_count);
+  return I4G_OK;
+}
+
+int i4g_route(const void* logits, int fp32_logits, int ld_logits, const float* bias, int T, int E,
+              int top_k, const i4g_route_t* options, int32_t* ids, float* weights,
+              int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace,
+              size_t workspace_bytes, void* stream) {
+  int st = check_route(T, E, top_k);
+  if (st != I4G_OK) return st;
+  if (!options || !offsets || (T > 0 && (!logits || !ids || !weights || !rows || !slots)))
+    return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  const i4g_route_t& o = *options;
+  if ((o.scoring != I4G_SCORE_SOFTMAX && o.scoring != I4G_SCORE_SIGMOID) ||
+      (o.group_score != I4G_GROUP_MAX && o.group_score != I4G_GROUP_TOP2))
+    return fail(I4G_ERR_VARIANT, "unknown scoring %d or group score %d", o.scoring,
+                o.group_score);
+  if (o.n_group < 1 || o.n_group > i4g::route::kMaxGroups || E % o.n_group != 0 ||
+      o.topk_group < 1 || o.topk_group > o.n_group)
+    return fail(I4G_ERR_SHAPE, "%d of %d groups of %d experts", o.topk_group, o.n_group, E);
+  if (top_k > o.topk_group * (E / o.n_group))
+    return fail(I4G_ERR_SHAPE, "top_k=%d of the %d experts in %d groups", top_k,
+                o.topk_group * (E / o.n_group), o.topk_group);
+  if (ld_logits < E) return fail(I4G_ERR_SHAPE, "ld_logits %d is less than E=%d", ld_logits, E);
+  if (!aligned(logits, fp32_logits ? 4 : 2) || !aligned(bias, 4) || !aligned(ids, 4) ||
+      !aligned(weights, 4) || !aligned(offsets, 4) || !aligned(rows, 4) || !aligned(slots, 4))
+    return fail(I4G_ERR_ALIGNMENT, "routing buffers must be aligned to their elements");
+  DeviceInfo* dev = nullptr;
+  if ((st = current_device(&dev)) != I4G_OK) return st;
+  const size_t need = i4g::route::workspace_bytes(T, E, dev->sm_count);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(I4G_ERR_SHAPE, "routing needs a 16-byte aligned workspace of %d bytes",
+                static_cast<int>(need));
+  i4g::route::Args a{};
+  a.logits = logits;
+  a.ld = static_cast<size_t>(ld_logits);
+  a.bias = bias;
+  a.T = T;
+  a.E = E;
+  a.top_k = top_k;
+  a.sigmoid = o.scoring == I4G_SCORE_SIGMOID;
+  a.n_group = o.n_group;
+  a.topk_group = o.topk_group;
+  a.top2 = o.group_score == I4G_GROUP_TOP2;
+  a.renormalize = o.renormalize;
+  a.scale = o.scale;
+  a.ids = ids;
+  a.weights = weights;
+  a.offsets = offsets;
+  a.rows = rows;
+  a.slots = slots;
+  return finish(i4g::route::launch(a, fp32_logits != 0, dev->sm_count, workspace,
+                                   static_cast<cudaStream_t>(stream)),
+                "routing launch");
+}
+
+int i4g_experts_combine(const void* y, int y_rows, const int32_t* slots, const float* weights,
+                        const void* residual, void* out, int T, int top_k, int N, void* stream) {
+  if (T < 0 || y_rows < 0 || top_k < 1 || N < 8 || N % 8 != 0 ||
+      static_cast<long long>(T) * top_k >= (1ll << 31))
+    return fail(I4G_ERR_SHAPE, "combine T=%d top_k=%d N=%d: N %% 8 == 0", T, top_k, N);
+  if (T == 0) return I4G_OK;
+  if ((!y && y_rows > 0) || !slots || !weights || !out)
+    return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  if (!aligned(y, 16) || !aligned(residual, 16) || !aligned(out, 16) || !aligned(slots, 4) ||
+      !aligned(weights, 4))
+    return fail(I4G_ERR_ALIGNMENT, "combine needs 16-byte aligned y, residual and out");
+  DeviceInfo* dev = nullptr;
+  const int st = current_device(&dev);
+  if (st != I4G_OK) return st;
+  return finish(i4g::route::combine(static_cast<const __half*>(y), y_rows, slots, weights,
+                                    static_cast<const __half*>(residual),
+                                    static_cast<__half*>(out), T, top_k, N,
+                                    static_cast<cudaStream_t>(stream)),
+                "combine launch");
 }
 
 int i4g_ipc_handle(const void* ptr, void* handle, size_t* offset) {

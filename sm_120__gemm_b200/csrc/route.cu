@@ -1,0 +1,551 @@
+// Routing to experts, the order of the routed rows, and their combination.
+//
+// Scores of a token: p_e = exp(x_e - max x) / sum (softmax) or
+// 1 / (1 + exp(-x_e)) (sigmoid). Its choice score is c_e = p_e + bias_e, or the
+// logit itself where nothing but the order of the p matters (no bias, no sum
+// of group members): the scores rise with the logits, so the order is the
+// same and exact. With groups, a group's score is its best member's c, or the
+// sum of its best two; only members of the topk_group best groups stay. The
+// top_k experts are those of the largest c, ties going to the lowest index;
+// their weights are the p (without bias), renormalised to sum 1 if asked,
+// times a factor. A logit of -infinity or NaN takes an expert out: its score
+// is 0 and it is never chosen (nor is one whose bias is -infinity or NaN); a
+// token with fewer than top_k experts left gets id -1 and weight 0 in the
+// places that stay empty.
+//
+// Exactness of the choice. FP32 scores that differ by a few rounding errors
+// may come out in either order, so a choice by scores is made in FP32 first
+// and redone in FP64 (for that token alone) when two neighbours in the order,
+// or the last group in and the first group out, are closer than the FP32
+// error. Few tokens need it, so the choice costs FP32 and is the one the
+// definition gives in FP64.
+//
+// One warp per token. Lane l holds experts l V .. l V + V - 1 (V = E / 32
+// rounded up), so among equal scores the lowest lane, and in it the lowest
+// register, is the lowest index. A round of the top-k is one warp-wide
+// maximum of order-preserving integer keys and a ballot.
+#include "route.h"
+
+#include "ptx.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+namespace i4g {
+namespace route {
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kChunk = 128;       // tokens whose choices one bitmap holds
+constexpr int kThreads = 1024;
+constexpr int kOneBlock = 128;    // up to so many tokens one CTA does everything
+
+// Order-preserving keys: larger value, larger key; 0 is "not eligible".
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and 0 are equal
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(double v) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+__device__ __forceinline__ double value_of(uint64_t k) {
+  return __longlong_as_double(
+      static_cast<long long>((k >> 63) ? (k ^ 0x8000000000000000ull) : ~k));
+}
+__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(kAll, k); }
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+  const uint32_t hi = static_cast<uint32_t>(k >> 32);
+  const uint32_t top = __reduce_max_sync(kAll, hi);
+  const uint32_t lo = __reduce_max_sync(kAll, hi == top ? static_cast<uint32_t>(k) : 0u);
+  return (static_cast<uint64_t>(top) << 32) | lo;
+}
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
+  return v;
+}
+
+template <typename F> struct Key;
+template <> struct Key<float> { using type = uint32_t; };
+template <> struct Key<double> { using type = uint64_t; };
+
+// The scores p of this lane's experts (0 where not eligible).
+template <typename F, int V>
+__device__ __forceinline__ void scores(const float (&x)[V], float top, int sigmoid, F (&p)[V]) {
+  if (sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      p[v] = x[v] > -INFINITY ? F(1) / (F(1) + exp_of(-static_cast<F>(x[v]))) : F(0);
+    return;
+  }
+  F sum = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    // the largest logit's term is 1, an infinite one's too
+    p[v] = x[v] > -INFINITY
+               ? (x[v] == top ? F(1) : exp_of(static_cast<F>(x[v]) - static_cast<F>(top)))
+               : F(0);
+    sum += p[v];
+  }
+  sum = warp_sum(sum);
+  const F r = sum > 0 ? F(1) / sum : F(0);
+#pragma unroll
+  for (int v = 0; v < V; ++v) p[v] *= r;
+}
+
+// The choice of one token. On return lane i < top_k holds the i-th expert
+// (or -1). Returns false when values closer than `tol` (relative to
+// max(1, |value|)) decided it; tol = 0 accepts every order.
+template <typename F, int V>
+__device__ __forceinline__ bool choose(const Args& a, int lane, const float (&x)[V],
+                                       const F (&p)[V], bool by_score, F tol, int& my_id) {
+  using K = typename Key<F>::type;
+  K key[V];
+  const int e0 = lane * V;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const F c = by_score ? p[v] + (a.bias && e0 + v < a.E ? static_cast<F>(a.bias[e0 + v]) : F(0))
+                         : static_cast<F>(x[v]);
+    key[v] = x[v] > -INFINITY && c > -INFINITY ? key_of(c) : K(0);
+  }
+  bool sure = true;
+  if (a.n_group > 1) {
+    const int size = a.E / a.n_group;
+    // Group scores: lane g holds group g's. A group may start and end inside
+    // a lane, so each group is a pass over the warp.
+    F mine = -INFINITY;
+    for (int g = 0; g < a.n_group; ++g) {
+      K best = 0, second = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int e = e0 + v;
+        const K k = e >= g * size && e < (g + 1) * size ? key[v] : K(0);
+        if (k > best) {
+          second = best;
+          best = k;
+        } else if (k > second) {
+          second = k;
+        }
+      }
+      const K top = warp_max(best);
+      F score = top ? value_of(top) : -INFINITY;
+      if (a.top2) {
+        const unsigned holders = __ballot_sync(kAll, best == top);
+        const K next = warp_max(lane == __ffs(holders) - 1 ? second : best);
+        if (next) score += value_of(next);
+      }
+      if (lane == g) mine = score;
+    }
+    int rank = 0;
+    F lowest_in = INFINITY, highest_out = -INFINITY;
+    for (int g = 0; g < a.n_group; ++g) {
+      const F other = __shfl_sync(kAll, mine, g);
+      rank += other > mine || (other == mine && g < lane);
+    }
+    const bool kept = lane < a.n_group && rank < a.topk_group;
+    const unsigned in = __ballot_sync(kAll, kept);
+    for (int g = 0; g < a.n_group; ++g) {
+      const F s = __shfl_sync(kAll, mine, g);
+      if ((in >> g) & 1) lowest_in = s < lowest_in ? s : lowest_in;
+      else highest_out = s > highest_out ? s : highest_out;
+    }
+    if (tol > 0 && highest_out > -INFINITY && by_score) {
+      const F size_of = fmax(F(1), fabs(lowest_in));
+      sure = lowest_in - highest_out > 2 * tol * size_of;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = e0 + v;
+      if (e < a.E && !((in >> (e / size)) & 1)) key[v] = 0;
+    }
+  }
+  my_id = -1;
+  K last = 0;
+  const int rounds = a.top_k + (tol > 0 && by_score ? 1 : 0);
+  for (int i = 0; i < rounds; ++i) {
+    K best = 0;
+    int at = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (key[v] > best) {
+        best = key[v];
+        at = v;
+      }
+    const K top = warp_max(best);
+    if (top == 0) break;  // none left
+    if (tol > 0 && by_score && i > 0) {
+      const F hi = value_of(last), lo = value_of(top);
+      if (!(hi - lo > tol * fmax(F(1), fabs(hi)))) sure = false;
+    }
+    last = top;
+    const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
+    const int id = __shfl_sync(kAll, e0 + at, winner);
+    if (lane == i && i < a.top_k) my_id = id;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (lane == winner && v == at) key[v] = 0;
+  }
+  return sure;
+}
+
+// Token t's experts and weights, by one warp; lane i < top_k returns expert i.
+template <int V, bool FP32>
+__device__ __forceinline__ int route_token(const Args& a, int t, int lane) {
+  float x[V];
+  const int e0 = lane * V;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    x[v] = -INFINITY;
+    if (e0 + v < a.E) {
+      const size_t at = static_cast<size_t>(t) * a.ld + e0 + v;
+      x[v] = FP32 ? static_cast<const float*>(a.logits)[at]
+                  : __half2float(static_cast<const __half*>(a.logits)[at]);
+    }
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < V; ++v) top = x[v] > top ? x[v] : top;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
+  float p[V];
+  scores(x, top, a.sigmoid, p);
+  const bool by_score = a.bias || (a.n_group > 1 && a.top2);
+  int id;
+  if (!choose(a, lane, x, p, by_score, 2e-6f, id)) {
+    double pd[V];
+    scores(x, top, a.sigmoid, pd);
+    choose(a, lane, x, pd, by_score, 0.0, id);
+  }
+  // lane i's weight is expert id's p
+  float w = 0.0f;
+  for (int i = 0; i < a.top_k; ++i) {
+    const int want = __shfl_sync(kAll, id, i);
+    if (want < 0) break;
+    float mine = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (e0 + v == want) mine = p[v];
+    mine = __shfl_sync(kAll, mine, want / V);
+    if (lane == i) w = mine;
+  }
+  if (a.renormalize) {
+    const float sum = warp_sum(lane < a.top_k ? w : 0.0f);
+    w = sum > 0.0f ? w / sum : 0.0f;
+  }
+  if (lane < a.top_k) {
+    const size_t at = static_cast<size_t>(t) * a.top_k + lane;
+    a.ids[at] = id;
+    a.weights[at] = w * a.scale;
+  }
+  return id;
+}
+
+// Tokens of block b of nb: [b T / nb, (b + 1) T / nb).
+__device__ __forceinline__ int first_token(int T, int b, int nb) {
+  return static_cast<int>(static_cast<long long>(b) * T / nb);
+}
+
+// A CTA's shared tables while it places pairs.
+struct Place {
+  int base[kMaxExperts];                      // next row of each expert
+  uint32_t bits[kMaxExperts][kChunk / 32];    // tokens of the chunk that chose it
+  int warp_total[32];
+};
+
+// Exclusive sum of v over the threads of the CTA (v = 0 past E); also the total.
+__device__ __forceinline__ int block_scan(int v, int* warp_total, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(kAll, sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 31) warp_total[warp] = sum;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) {
+    if (i < warp) before += warp_total[i];
+    total += warp_total[i];
+  }
+  return before + sum - v;
+}
+
+// Gives the pairs of tokens [t0, t1) their rows: an expert's next row is
+// base[e]; inside a chunk of kChunk tokens a pair's place is the number of
+// earlier tokens that chose the same expert, counted in the expert's bitmap
+// (a token chooses an expert once), so the order is by token and nothing
+// depends on which thread comes first.
+__device__ __forceinline__ void place_pairs(const Args& a, Place& s, int t0, int t1) {
+  for (int c0 = t0; c0 < t1; c0 += kChunk) {
+    const int n = min(kChunk, t1 - c0);
+    for (int i = threadIdx.x; i < a.E * (kChunk / 32); i += blockDim.x)
+      (&s.bits[0][0])[i] = 0u;
+    __syncthreads();
+    const int pairs = n * a.top_k;
+    const size_t p0 = static_cast<size_t>(c0) * a.top_k;
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+      const int e = a.ids[p0 + i], t = i / a.top_k;
+      if (e >= 0) atomicOr(&s.bits[e][t >> 5], 1u << (t & 31));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+      const int e = a.ids[p0 + i], t = i / a.top_k;
+      int row = -1;
+      if (e >= 0) {
+        row = s.base[e] + __popc(s.bits[e][t >> 5] & ((1u << (t & 31)) - 1u));
+        for (int q = 0; q < (t >> 5); ++q) row += __popc(s.bits[e][q]);
+        a.rows[row] = static_cast<int>(p0) + i;
+      }
+      a.slots[p0 + i] = row;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+      int count = 0;
+#pragma unroll
+      for (int q = 0; q < kChunk / 32; ++q) count += __popc(s.bits[e][q]);
+      s.base[e] += count;
+    }
+    __syncthreads();
+  }
+}
+
+// Everything in one CTA (T <= kOneBlock).
+template <int V, bool FP32>
+__global__ void __launch_bounds__(kThreads, 1) route_small_kernel(const Args a) {
+  __shared__ Place s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) s.base[e] = 0;
+  grid_dependency_wait();
+  if (threadIdx.x == 0) launch_dependents();
+  __syncthreads();
+  for (int t = warp; t < a.T; t += blockDim.x / 32) {
+    const int e = route_token<V, FP32>(a, t, lane);
+    if (lane < a.top_k && e >= 0) atomicAdd(&s.base[e], 1);
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  int total;
+  const int before = block_scan(e < a.E ? s.base[e] : 0, s.warp_total, total);
+  __syncthreads();
+  if (e < a.E) {
+    s.base[e] = before;
+    a.offsets[e] = before;
+  }
+  if (e == 0) a.offsets[a.E] = total;
+  __syncthreads();
+  place_pairs(a, s, 0, a.T);
+  for (int i = total + threadIdx.x; i < a.T * a.top_k; i += blockDim.x) a.rows[i] = -1;
+}
+
+// First of two kernels: choices, and how many of the block's pairs each
+// expert got (counts [block][E], 16 bits each: a block has fewer tokens).
+template <int V, bool FP32>
+__global__ void __launch_bounds__(kThreads, 1)
+    route_choose_kernel(const Args a, uint16_t* __restrict__ counts) {
+  __shared__ int count[kMaxExperts];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) count[e] = 0;
+  grid_dependency_wait();
+  if (threadIdx.x == 0) launch_dependents();
+  __syncthreads();
+  const int t0 = first_token(a.T, blockIdx.x, gridDim.x);
+  const int t1 = first_token(a.T, blockIdx.x + 1, gridDim.x);
+  for (int t = t0 + warp; t < t1; t += blockDim.x / 32) {
+    const int e = route_token<V, FP32>(a, t, lane);
+    if (lane < a.top_k && e >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x)
+    counts[static_cast<size_t>(blockIdx.x) * a.E + e] = static_cast<uint16_t>(count[e]);
+}
+
+// Second kernel: every block adds the counts up itself (all of them for the
+// experts' offsets, those of earlier blocks for its own first rows), then
+// places its tokens' pairs. The counts are a few tens of KB in L2.
+__global__ void __launch_bounds__(kThreads, 1)
+    route_place_kernel(const Args a, const uint16_t* __restrict__ counts) {
+  __shared__ Place s;
+  __shared__ int all[kMaxExperts];
+  for (int e = threadIdx.x; e < kMaxExperts; e += blockDim.x) s.base[e] = all[e] = 0;
+  grid_dependency_wait();
+  if (threadIdx.x == 0) launch_dependents();
+  __syncthreads();
+  const int nb = gridDim.x, b = blockIdx.x;
+  const int lanes = max(1, static_cast<int>(blockDim.x) / a.E);  // threads per expert
+  const int e = threadIdx.x % a.E, part = threadIdx.x / a.E;
+  if (part < lanes) {
+    int before = 0, sum = 0;
+#pragma unroll 8
+    for (int i = part; i < nb; i += lanes) {
+      const int c = counts[static_cast<size_t>(i) * a.E + e];
+      sum += c;
+      before += i < b ? c : 0;
+    }
+    atomicAdd(&all[e], sum);  // integers: the order does not matter
+    atomicAdd(&s.base[e], before);
+  }
+  __syncthreads();
+  int total;
+  const int mine = threadIdx.x;
+  const int first = block_scan(mine < a.E ? all[mine] : 0, s.warp_total, total);
+  if (mine < a.E) {
+    s.base[mine] += first;
+    if (b == 0) a.offsets[mine] = first;
+  }
+  if (b == 0 && mine == 0) a.offsets[a.E] = total;
+  __syncthreads();
+  place_pairs(a, s, first_token(a.T, b, nb), first_token(a.T, b + 1, nb));
+  const size_t pairs = static_cast<size_t>(a.T) * a.top_k;
+  for (size_t i = total + static_cast<size_t>(b) * blockDim.x + threadIdx.x; i < pairs;
+       i += static_cast<size_t>(nb) * blockDim.x)
+    a.rows[i] = -1;
+}
+
+int blocks_for(int T, int sm_count) {
+  // one block per SM; more only so that a block's counts fit 16 bits
+  const int most = std::max(sm_count, (T + 32767) / 32768);
+  return std::min(most, (T + 31) / 32);
+}
+
+template <typename... KArgs, typename... AArgs>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), int grid, int threads, cudaStream_t stream,
+                             AArgs... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int V, bool FP32>
+cudaError_t launch_typed(const Args& a, int sm_count, void* workspace, cudaStream_t stream) {
+  if (a.T <= kOneBlock)
+    return launch_dependent(route_small_kernel<V, FP32>, 1, kThreads, stream, a);
+  uint16_t* counts = static_cast<uint16_t*>(workspace);
+  const int nb = blocks_for(a.T, sm_count);
+  cudaError_t e = launch_dependent(route_choose_kernel<V, FP32>, nb, kThreads, stream, a, counts);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(route_place_kernel, nb, kThreads, stream, a,
+                          static_cast<const uint16_t*>(counts));
+}
+
+// out[t] = residual[t] + sum_s w[t, s] y[slots[t, s]]: a thread does eight
+// columns of one token in FP32, in slot order, with the rows' loads issued
+// together. Bound by the bytes of y.
+constexpr int kCombineThreads = 128;
+
+__global__ void __launch_bounds__(kCombineThreads)
+    combine_kernel(const __half* __restrict__ y, int y_rows, const int* __restrict__ slots,
+                   const float* __restrict__ weights, const __half* residual, __half* out,
+                   int top_k, int N) {
+  grid_dependency_wait();
+  if (threadIdx.x == 0) launch_dependents();
+  const int col = (blockIdx.y * kCombineThreads + threadIdx.x) * 8;
+  const size_t t = blockIdx.x;
+  if (col >= N) return;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+  constexpr int BATCH = 8;
+  for (int s0 = 0; s0 < top_k; s0 += BATCH) {
+    uint4 v[BATCH];
+    float w[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int slot = s0 + b < top_k ? slots[t * top_k + s0 + b] : -1;
+      const bool has = static_cast<unsigned>(slot) < static_cast<unsigned>(y_rows);
+      w[b] = has ? weights[t * top_k + s0 + b] : 0.0f;
+      v[b] = has ? *reinterpret_cast<const uint4*>(y + static_cast<size_t>(slot) * N + col)
+                 : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const uint32_t q[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(u32_as_half2(q[i]));
+        acc[2 * i] = fmaf(w[b], f.x, acc[2 * i]);
+        acc[2 * i + 1] = fmaf(w[b], f.y, acc[2 * i + 1]);
+      }
+    }
+  }
+  if (residual) {
+    const uint4 r = *reinterpret_cast<const uint4*>(residual + t * N + col);
+    const uint32_t q[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(u32_as_half2(q[i]));
+      acc[2 * i] += f.x;
+      acc[2 * i + 1] += f.y;
+    }
+  }
+  uint4 o;
+  o.x = half2_as_u32(__floats2half2_rn(acc[0], acc[1]));
+  o.y = half2_as_u32(__floats2half2_rn(acc[2], acc[3]));
+  o.z = half2_as_u32(__floats2half2_rn(acc[4], acc[5]));
+  o.w = half2_as_u32(__floats2half2_rn(acc[6], acc[7]));
+  *reinterpret_cast<uint4*>(out + t * N + col) = o;
+}
+
+}  // namespace
+
+size_t workspace_bytes(int T, int E, int sm_count) {
+  if (T <= kOneBlock) return 0;
+  return static_cast<size_t>(blocks_for(T, sm_count)) * E * sizeof(uint16_t);
+}
+
+cudaError_t launch(const Args& a, bool fp32_logits, int sm_count, void* workspace,
+                   cudaStream_t stream) {
+  const int v = (a.E + 31) / 32;
+#define I4G_ROUTE_CASE(V)                                                          \
+  if (v <= V)                                                                      \
+    return fp32_logits ? launch_typed<V, true>(a, sm_count, workspace, stream)     \
+                       : launch_typed<V, false>(a, sm_count, workspace, stream);
+  I4G_ROUTE_CASE(1)
+  I4G_ROUTE_CASE(2)
+  I4G_ROUTE_CASE(4)
+  I4G_ROUTE_CASE(8)
+  I4G_ROUTE_CASE(16)
+#undef I4G_ROUTE_CASE
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t combine(const __half* y, int y_rows, const int* slots, const float* weights,
+                    const __half* residual, __half* out, int T, int top_k, int N,
+                    cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(T, (N / 8 + kCombineThreads - 1) / kCombineThreads);
+  cfg.blockDim = dim3(kCombineThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel, y, y_rows, slots, weights, residual, out, top_k,
+                            N);
+}
+
+}  // namespace route
+}  // namespace i4g

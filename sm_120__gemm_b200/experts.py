@@ -1,0 +1,219 @@
+"""A mixture of experts over INT4 weights: routing, the experts' products and
+their combination.
+
+    r = route(logits, top_k=8)                       # [T, E] -> experts, order
+    h = gate_up(x, r, activation="silu", gated=True)  # [T * 8, F], expert order
+    y = down(h, r, gather=False)                     # [T * 8, N], expert order
+    out = combine(y, r, residual=x)                  # [T, N]
+
+(``ExpertMLP`` is those four calls.) Nothing is read back to the host: the
+number of rows an expert gets stays on the device, and every buffer has
+T * top_k rows whatever the routing is. Rows behind the last expert's (tokens
+routed to fewer than top_k experts) are left as they were.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import (ACTIVATIONS, GROUP_SCORES, SCORINGS, RouteOptions, experts_workspace_size,
+               launch_combine, launch_experts, launch_quantize_repack, launch_repack_scales_128,
+               launch_repack_umma, launch_route, route_workspace_size)
+from .launching import on, want, want_out, workspace
+from .linear import interleave_gate_up
+
+
+class Routing(NamedTuple):
+    """A batch's routing. A pair is token * top_k + place."""
+    ids: torch.Tensor      # int32 [T, top_k]: experts, best first (-1: none)
+    weights: torch.Tensor  # float32 [T, top_k]
+    offsets: torch.Tensor  # int32 [E + 1]: expert e has sorted rows offsets[e] .. offsets[e + 1]
+    rows: torch.Tensor     # int32 [T * top_k]: the pair of each sorted row (-1 past the last)
+    slots: torch.Tensor    # int32 [T, top_k]: the sorted row of each pair (-1: none)
+
+
+def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
+          bias: torch.Tensor | None = None, n_group: int = 1, topk_group: int = 1,
+          group_score: str = "max", renormalize: bool = True, scale: float = 1.0,
+          stream=None) -> Routing:
+    """Each token's ``top_k`` experts from its logits [T, E] (float32 or
+    float16, rows of any stride), as C ABI i4g_route describes: softmax or
+    sigmoid scores, ``bias`` (float32 [E]) added for the choice only, the best
+    ``topk_group`` of ``n_group`` groups, ties to the lowest index, weights
+    renormalised to sum 1 and scaled."""
+    if scoring not in SCORINGS or group_score not in GROUP_SCORES:
+        raise ValueError(f"unknown scoring {scoring!r} or group_score {group_score!r}")
+    want(logits, "logits", (torch.float32, torch.float16))
+    if logits.dim() != 2:
+        raise ValueError("logits must be [T, E]")
+    T, E = logits.shape
+    dev = logits.device
+    with on(dev, stream, logits, bias):
+        if logits.stride(1) != 1 or logits.stride(0) < E:
+            logits = logits.contiguous()
+        if bias is not None:
+            bias = want(bias, "bias", torch.float32, (E,), dev).contiguous()
+        pairs = T * top_k
+        # one allocation: ids, slots, rows, offsets (int32) and weights (float32)
+        buf = torch.empty(4 * pairs + E + 1, dtype=torch.int32, device=dev)
+        ids, weights, slots, rows, offsets = buf.split((pairs, pairs, pairs, pairs, E + 1))
+        r = Routing(ids.view(T, top_k), weights.view(torch.float32).view(T, top_k), offsets, rows,
+                    slots.view(T, top_k))
+        options = RouteOptions(SCORINGS[scoring], n_group, topk_group, GROUP_SCORES[group_score],
+                               bool(renormalize), scale)
+        need = route_workspace_size(T, E)  # for its counts; nothing is kept in it
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        launch_route(logits, logits.dtype == torch.float32, logits.stride(0) if T > 1 else E, bias,
+                     T, E, top_k, options, r.ids, r.weights, r.offsets, r.rows, r.slots, ws)
+    return r
+
+
+def combine(y: torch.Tensor, routing: Routing, *, residual: torch.Tensor | None = None,
+            out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """out[t] = residual[t] + sum over places s of weights[t, s] * y[slots[t, s]]
+    (C ABI i4g_experts_combine): y fp16 in expert order, out fp16 [T, N]."""
+    want(y, "y", torch.float16)
+    dev = y.device
+    weights, slots = routing.weights, routing.slots
+    T, top_k = slots.shape
+    want_out(slots, "routing.slots", torch.int32, (T, top_k), dev)
+    want_out(weights, "routing.weights", torch.float32, (T, top_k), dev)
+    if y.dim() != 2:
+        raise ValueError("y must be [rows, N]")
+    N = y.shape[1]
+    if out is not None:
+        want_out(out, "out", torch.float16, (T, N), dev)
+    with on(dev, stream, y, weights, slots, residual, out):
+        y = y.contiguous()
+        if residual is not None:
+            residual = want(residual, "residual", torch.float16, (T, N), dev).contiguous()
+        if out is None:
+            out = torch.empty(T, N, dtype=torch.float16, device=dev)
+        launch_combine(y, y.shape[0], slots, weights, residual, out, T, top_k, N)
+    return out
+
+
+class QuantizedExperts:
+    """E experts' INT4 weights of one [K, N], one after another in the GEMM's layouts."""
+
+    def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, E: int, K: int, N: int,
+                 group: int):
+        if tiles.dtype != torch.uint8 or scales.dtype != torch.float16:
+            raise TypeError("tiles must be uint8 and scales float16")
+        if tiles.numel() != E * (K * N // 2) or scales.numel() != E * (K // group) * N:
+            raise ValueError("buffer sizes do not match E, K, N, group")
+        if not tiles.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("tiles and scales must be contiguous")
+        self.tiles, self.scales = tiles.view(E, -1), scales.view(E, -1)
+        self.E, self.K, self.N, self.group = E, K, N, group
+
+    @classmethod
+    def _empty(cls, E, K, N, group, device):
+        tiles = torch.empty(E, K * N // 2, dtype=torch.uint8, device=device)
+        scales = torch.empty(E, (K // group) * N, dtype=torch.float16, device=device)
+        return cls(tiles, scales, E, K, N, group)
+
+    @classmethod
+    def from_weight(cls, w: torch.Tensor, group: int, stream=None) -> "QuantizedExperts":
+        """Quantise fp16 [E, K, N] weights, each as QuantizedLinear.from_weight does."""
+        want(w, "weight", torch.float16)
+        if w.dim() != 3:
+            raise ValueError("weight must be [E, K, N]")
+        E, K, N = w.shape
+        with on(w.device, stream, w):
+            self = cls._empty(E, K, N, group, w.device)
+            for e in range(E):
+                launch_quantize_repack(w[e].contiguous(), self.tiles[e], self.scales[e], K, N,
+                                       group)
+        return self
+
+    @classmethod
+    def from_gate_up(cls, gate: torch.Tensor, up: torch.Tensor, group: int,
+                     stream=None) -> "QuantizedExperts":
+        """One weight per expert of the fp16 [E, K, F] gate and up projections, for
+        calls with gated=True."""
+        return cls.from_weight(interleave_gate_up(gate, up), group, stream)
+
+    @classmethod
+    def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, K: int, N: int, group: int,
+                    stream=None) -> "QuantizedExperts":
+        """Repack quantiser-layout codes [E][K * N / 2] and scales [E][K / group][N]."""
+        want(packed, "packed", torch.uint8)
+        E, dev = packed.shape[0], packed.device
+        want(scales, "scales", torch.float16, None, dev)
+        if packed.numel() != E * (K * N // 2) or scales.numel() != E * (K // group) * N:
+            raise ValueError("buffer sizes do not match E, K, N, group")
+        with on(dev, stream, packed, scales):
+            self = cls._empty(E, K, N, group, dev)
+            packed, scales = packed.contiguous().view(E, -1), scales.contiguous().view(E, -1)
+            for e in range(E):
+                launch_repack_umma(packed[e], self.tiles[e], K, N)
+                launch_repack_scales_128(scales[e], self.scales[e], K, N, group)
+        return self
+
+    def __call__(self, a: torch.Tensor, routing: Routing, *, gather: bool = True,
+                 bias: torch.Tensor | None = None, activation: str = "none", gated: bool = False,
+                 out: torch.Tensor | None = None, fp32_out: bool = False,
+                 stream=None) -> torch.Tensor:
+        """The routed rows' products in expert order, [T * top_k, N] (gated: N / 2).
+        gather: ``a`` is the tokens' rows [T, K]; otherwise rows already in
+        expert order [T * top_k, K]. bias: fp16 [E, N]. Rows of the result past
+        routing.offsets[E] are left as they were."""
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}")
+        dev = self.tiles.device
+        want(a, "A", torch.float16, None, dev)
+        T, top_k = routing.slots.shape
+        pairs = T * top_k
+        want_out(routing.offsets, "routing.offsets", torch.int32, (self.E + 1,), dev)
+        want_out(routing.rows, "routing.rows", torch.int32, (pairs,), dev)
+        rows_a = T if gather else pairs
+        if a.dim() != 2 or a.shape[0] != rows_a or a.shape[1] != self.K:
+            raise ValueError(f"A must be float16 [{rows_a}, {self.K}]")
+        cols = self.N // 2 if gated else self.N
+        dtype = torch.float32 if fp32_out else torch.float16
+        if out is not None:
+            want_out(out, "out", dtype, (pairs, cols), dev)
+        with on(dev, stream, a, routing.offsets, routing.rows, bias, out):
+            a = a.contiguous()
+            if bias is not None:
+                bias = want(bias, "bias", torch.float16, (self.E, self.N), dev).contiguous()
+            if out is None:
+                out = torch.empty(pairs, cols, dtype=dtype, device=dev)
+            ws = workspace(_experts_workspace(dev, pairs, self.E, self.N, self.K), dev)
+            launch_experts(a, rows_a, self.tiles, self.scales, out, routing.offsets,
+                           routing.rows if gather else None, top_k, pairs, self.E, self.N, self.K,
+                           self.group, bias, activation, gated, fp32_out, ws)
+        return out
+
+
+class ExpertMLP:
+    """The gated MLP of a mixture of experts: gate and up projection
+    (``gate_up``: K -> 2 F, columns of ``from_gate_up``), activation, ``down``:
+    F -> K, weighted sum."""
+
+    def __init__(self, gate_up: QuantizedExperts, down: QuantizedExperts,
+                 activation: str = "silu"):
+        if gate_up.E != down.E or gate_up.N != 2 * down.K:
+            raise ValueError("gate_up [E, K, 2 F] and down [E, F, N] do not belong together")
+        self.gate_up, self.down, self.activation = gate_up, down, activation
+
+    def __call__(self, x: torch.Tensor, routing: Routing, *,
+                 residual: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        h = self.gate_up(x, routing, activation=self.activation, gated=True, stream=stream)
+        y = self.down(h, routing, gather=False, stream=stream)
+        return combine(y, routing, residual=residual, stream=stream)
+
+
+_sizes: dict = {}
+
+
+def _experts_workspace(device, pairs: int, E: int, N: int, K: int) -> int:
+    key = (device.index, pairs, E, N, K)
+    n = _sizes.get(key)
+    if n is None:
+        if len(_sizes) > 4096:  # calls of ever new sizes do not fill the memory
+            _sizes.clear()
+        n = _sizes[key] = experts_workspace_size(pairs, E, N, K)
+    return n

@@ -9,8 +9,20 @@ from __future__ import annotations
 
 import torch
 
-from . import (launch_final_fp32_ws, launch_final_ws, launch_quantize_repack,
+from . import (ACTIVATIONS, gemm_epilogue_workspace_size, launch_final_epilogue,
+               launch_final_fp32_ws, launch_final_ws, launch_quantize_repack,
                launch_repack_scales_128, launch_repack_umma, shard_range, workspace_for)
+from .launching import on, want, want_out, workspace
+
+
+def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """[..., F] gates and ups -> [..., 2 F] gated columns: groups of 16, eight
+    gates and then the eight columns they gate (weights or biases)."""
+    if gate.shape != up.shape or gate.shape[-1] % 8:
+        raise ValueError("gate and up need one shape and a multiple of 8 columns")
+    lead, F = gate.shape[:-1], gate.shape[-1]
+    both = torch.stack((gate.reshape(*lead, F // 8, 8), up.reshape(*lead, F // 8, 8)), dim=-2)
+    return both.reshape(*lead, 2 * F)
 
 
 class QuantizedLinear:
@@ -38,6 +50,13 @@ class QuantizedLinear:
         return cls(tiles, rscales, K, N, group)
 
     @classmethod
+    def from_gate_up(cls, gate: torch.Tensor, up: torch.Tensor, group: int,
+                     stream=None) -> "QuantizedLinear":
+        """One weight of the fp16 [K, F] gate and up projections, for calls with
+        gated=True (F % 64 == 0; a column's codes do not depend on its place)."""
+        return cls.from_weight(interleave_gate_up(gate, up), group, stream)
+
+    @classmethod
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, K: int, N: int,
                     group: int, stream=None) -> "QuantizedLinear":
         """Repack reference-layout codes ([K][N] nibbles) and scales ([K/g][N])."""
@@ -58,7 +77,15 @@ class QuantizedLinear:
         return QuantizedLinear(tiles, scales, self.K, n_local, self.group)
 
     def __call__(self, a: torch.Tensor, out: torch.Tensor | None = None, fp32_out: bool = False,
-                 stream=None) -> torch.Tensor:
+                 stream=None, *, bias: torch.Tensor | None = None, activation: str = "none",
+                 gated: bool = False, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """A x dequant(B), or with any of the keyword arguments the fused epilogue
+        (``launch_final_epilogue``): act(A x dequant(B) + bias) + residual, and with
+        ``gated`` (columns as ``from_gate_up`` lays them out) act(gate) * up with N / 2
+        columns. bias: fp16 [N]; residual: fp16, C's shape, rows of any stride (it may be
+        ``out``)."""
+        if bias is not None or residual is not None or gated or activation != "none":
+            return self._epilogue(a, out, fp32_out, stream, bias, activation, gated, residual)
         if a.dtype != torch.float16 or a.dim() != 2 or a.shape[1] != self.K:
             raise ValueError(f"A must be float16 [M, {self.K}]")
         a = a.contiguous()
@@ -70,3 +97,44 @@ class QuantizedLinear:
         fn = launch_final_fp32_ws if fp32_out else launch_final_ws
         fn(a, self.tiles, self.scales, out, M, self.N, self.K, self.group, ws, stream)
         return out
+
+    def _epilogue(self, a, out, fp32_out, stream, bias, activation, gated, residual):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}")
+        dev = self.tiles.device
+        want(a, "A", torch.float16, None, dev)
+        if a.dim() != 2 or a.shape[1] != self.K:
+            raise ValueError(f"A must be float16 [M, {self.K}]")
+        M, cols = a.shape[0], self.N // 2 if gated else self.N
+        dtype = torch.float32 if fp32_out else torch.float16
+        if out is not None:
+            want_out(out, "out", dtype, (M, cols), dev)
+        with on(dev, stream, a, bias, residual, out):
+            a = a.contiguous()
+            ld = 0
+            if bias is not None:
+                bias = want(bias, "bias", torch.float16, (self.N,), dev).contiguous()
+            if residual is not None:
+                want(residual, "residual", torch.float16, (M, cols), dev)
+                if residual.stride(1) != 1 or residual.stride(0) < cols:
+                    residual = residual.contiguous()
+                ld = residual.stride(0)
+            if out is None:
+                out = torch.empty(M, cols, dtype=dtype, device=dev)
+            ws = workspace(_epilogue_workspace(dev, M, self.N, self.K), dev)
+            launch_final_epilogue(a, self.tiles, self.scales, out, M, self.N, self.K, self.group,
+                                  bias, activation, gated, residual, ld, fp32_out, ws)
+        return out
+
+
+_sizes: dict = {}
+
+
+def _epilogue_workspace(device, M: int, N: int, K: int) -> int:
+    key = (device.index, M, N, K)
+    n = _sizes.get(key)
+    if n is None:
+        if len(_sizes) > 4096:  # calls of ever new sizes do not fill the memory
+            _sizes.clear()
+        n = _sizes[key] = gemm_epilogue_workspace_size(M, N, K)
+    return n
