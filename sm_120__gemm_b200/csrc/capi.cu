@@ -305,19 +305,24 @@ int gemm_common(const void* A, const uint8_t* tiles, const void* scales, const i
                 "tcgen05 kernel launch");
 }
 
-// Activation map of the epilogue / experts kernel: A [rows][K] fp16, 128-byte
-// swizzle, box 64 (K) x box_rows (1 for the row gather), zeros outside.
-int epi_map(const void* A, int rows, int K, int box_rows, CUtensorMap* map) {
+// Activation map of the epilogue / experts kernel, 128-byte swizzle, zeros
+// outside: A [rows][K] fp16 seen as {64 k, rows, K / 64 blocks} with a box of
+// box_rows rows x box_blocks blocks, or (box_rows 0, the row gather) as
+// {K, rows} with a box of 64 k x 1 row.
+int epi_map(const void* A, int rows, int K, int box_rows, int box_blocks, CUtensorMap* map) {
   EncodeTiledFn encode = nullptr;
   const int st = encode_fn(&encode);
   if (st != I4G_OK) return st;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t estr[2] = {1, 1};
+  const bool gather = box_rows == 0;
+  const cuuint64_t n = static_cast<cuuint64_t>(rows), k = static_cast<cuuint64_t>(K);
+  const cuuint64_t dims[3] = {gather ? k : 64, n, k / 64};
+  const cuuint64_t strides[2] = {k * 2, 128};
+  const cuuint32_t box[3] = {64, gather ? 1u : static_cast<cuuint32_t>(box_rows),
+                             static_cast<cuuint32_t>(box_blocks)};
+  const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r =
-      encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(A), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, gather ? 2 : 3, const_cast<void*>(A), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS
              ? I4G_OK
@@ -340,6 +345,16 @@ int check_epilogue(const i4g_epilogue_t& e, int N) {
 // Rows per weight that choose the tile height of an experts' product: the
 // mean over the experts that can have any.
 int mean_rows(int pairs, int E) { return (pairs + (pairs < E ? pairs : E) - 1) / (pairs < E ? pairs : E); }
+
+// Where a workspace holds the activations copied into row order (behind the
+// split tail's `split_bytes`, and behind the counters in any case), and the
+// workspace's size with them.
+size_t rows_offset(size_t split_bytes) {
+  return split_bytes > i4g::tc::kTicketBytes ? split_bytes : i4g::tc::kTicketBytes;
+}
+size_t bytes_with_rows(size_t split_bytes, int pairs, int K) {
+  return rows_offset(split_bytes) + static_cast<size_t>(pairs) * K * 2;
+}
 
 // The checks and the launch that i4g_gemm_epilogue (offsets null) and
 // i4g_experts_gemm share; pointers are checked by the caller.
@@ -364,10 +379,25 @@ int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scal
   if ((st = current_device(&dev)) != I4G_OK) return st;
   const int tile_m = i4g::epi::choose_tile(offsets ? mean_rows(M, E) : M);
   const long tiles_most = i4g::epi::tiles_bound(tile_m, M, E, N);
+  // the workspace holds the split tail's part, then the activations in row
+  // order where they are copied; each is used if it fits
   const size_t need = i4g::epi::workspace_bytes(tile_m, tiles_most, K, dev->sm_count);
   const bool split = workspace && need > 0 && workspace_bytes >= need;
+  if (rows && tile_m >= i4g::epi::kCopyRowsTile && workspace &&
+      workspace_bytes >= bytes_with_rows(need, M, K)) {
+    __half* copy = reinterpret_cast<__half*>(static_cast<char*>(workspace) + rows_offset(need));
+    const cudaError_t g = i4g::epi::gather_rows(static_cast<const __half*>(A), a_rows, offsets,
+                                                rows, row_div, copy, M, E, K, dev->sm_count,
+                                                static_cast<cudaStream_t>(stream));
+    if (g != cudaSuccess) return record_cuda(g, "row gather launch");
+    A = copy;
+    a_rows = M;
+    rows = nullptr;
+  }
   CUtensorMap map;
-  if ((st = epi_map(A, a_rows, K, rows ? 1 : tile_m, &map)) != I4G_OK) return st;
+  if ((st = epi_map(A, a_rows, K, rows ? 0 : tile_m, i4g::epi::box_blocks(tile_m), &map)) !=
+      I4G_OK)
+    return st;
   i4g::epi::Args args{};
   args.tiles = tiles;
   args.scales = static_cast<const __half*>(scales);
@@ -773,6 +803,7 @@ int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes) {
   const int tile_m = i4g::epi::choose_tile(mean_rows(pairs, E));
   *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, pairs, E, N), K,
                                      dev->sm_count);
+  if (tile_m >= i4g::epi::kCopyRowsTile) *bytes = bytes_with_rows(*bytes, pairs, K);
   return I4G_OK;
 }
 

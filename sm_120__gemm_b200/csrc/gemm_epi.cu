@@ -12,6 +12,60 @@ int choose_tile(int rows) {
   return 256;
 }
 
+int box_blocks(int tile_m) {
+  switch (tile_m) {
+    case 16: return Cfg<16>::BS;
+    case 32: return Cfg<32>::BS;
+    case 64: return Cfg<64>::BS;
+    case 128: return Cfg<128>::BS;
+    default: return Cfg<256>::BS;
+  }
+}
+
+namespace {
+
+// One row per warp, 16 bytes a lane: bound by the bytes it writes. The row
+// gather inside the product costs about 70 cycles of the copy unit for four
+// rows of 128 bytes, which for 64 rows a tile is more than the block's MMAs.
+constexpr int kGatherThreads = 256;
+
+__global__ void __launch_bounds__(kGatherThreads)
+    gather_rows_kernel(const __half* __restrict__ A, int a_rows, const int* __restrict__ offsets,
+                       const int* __restrict__ rows, int row_div, __half* __restrict__ out, int M,
+                       int E, int K) {
+  grid_dependency_wait();
+  if (threadIdx.x == 0) launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int end = min(max(offsets[E], 0), M);
+  const int warps = gridDim.x * (kGatherThreads / 32);
+  for (int p = blockIdx.x * (kGatherThreads / 32) + (threadIdx.x >> 5); p < end; p += warps) {
+    const int r = rows[p] / row_div;
+    const bool has = rows[p] >= 0 && r < a_rows;  // rows outside A read as zeros
+    const uint4* src = reinterpret_cast<const uint4*>(A + static_cast<size_t>(has ? r : 0) * K);
+    uint4* dst = reinterpret_cast<uint4*>(out + static_cast<size_t>(p) * K);
+#pragma unroll 8
+    for (int c = lane; c < K / 8; c += 32) dst[c] = has ? src[c] : make_uint4(0, 0, 0, 0);
+  }
+}
+
+}  // namespace
+
+cudaError_t gather_rows(const __half* A, int a_rows, const int* offsets, const int* rows,
+                        int row_div, __half* out, int M, int E, int K, int sm_count,
+                        cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(std::min(sm_count * 8, (M + kGatherThreads / 32 - 1) / (kGatherThreads / 32)));
+  cfg.blockDim = dim3(kGatherThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gather_rows_kernel, A, a_rows, offsets, rows, row_div, out, M, E,
+                            K);
+}
+
 long tiles_bound(int tile_m, int M, int E, int N) {
   // each expert's last tile may be partial, and no more experts than rows have any
   const long extra = std::min(E, M);

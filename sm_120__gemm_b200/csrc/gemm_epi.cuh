@@ -47,42 +47,50 @@ constexpr int BK = 64;
 constexpr int T_COLS = 32;                     // TMEM columns per weight stage
 constexpr int TMEM_COLS = 512;
 constexpr int WBLOCK_BYTES = TILE_N * BK / 2;  // 4096
-constexpr int W_SLOT = WBLOCK_BYTES + 512;     // + up to two groups of scales
 constexpr int FIRST_DEQ_WARP = 3;
 constexpr int kPromoteBlocks = 32;             // 2048 k, as gemm_tc.cu
 constexpr int kTableInts = kMaxExperts + 1 + 32;
 
 template <int TILE_M>
 struct Cfg {
-  static constexpr int DEQ = TILE_M <= 64 ? 3 : (TILE_M <= 128 ? 2 : 1);  // dequant groups
+    static constexpr int DEQ = TILE_M <= 128 ? 3 : 1;  // dequant groups
   static constexpr int PARTS = TILE_M <= 32 ? 1 : (TILE_M <= 128 ? 2 : 4);
   static constexpr int EPI_WARPS = 4 * PARTS;
   static constexpr int COLS = TILE_M / PARTS;  // accumulator columns per epilogue thread
   static constexpr int FIRST_EPI_WARP = FIRST_DEQ_WARP + 4 * DEQ;
   static constexpr int THREADS = 32 * (FIRST_EPI_WARP + EPI_WARPS);
   static constexpr int ACC = TILE_M <= 128 ? 2 : 1;
-  static constexpr int ACT_BYTES = TILE_M * BK * 2;
-  // a stage is one 64-k block: its activation box in shared memory and its
-  // 32 TMEM columns of dequantised weights, sharing one pair of barriers
-  static constexpr int STAGES = TILE_M <= 64 ? 9 : (TILE_M <= 128 ? 8 : 5);
-  static constexpr int ACC_COL = TILE_M <= 128 ? STAGES * T_COLS : 256;
+  // A stage is BS 64-k blocks: their activation boxes in shared memory and
+  // their 32 TMEM columns each of dequantised weights, sharing one pair of
+  // barriers. While three dequant warps keep a scheduler's half-rate pipes
+  // busy, every instruction of the warps that only issue copies and MMAs takes
+  // about 18 cycles, so a barrier round per block would bound the kernel;
+  // K = 65536, N = 18944, 16 rows: 185 us with two blocks a stage, 148 with four.
+  static constexpr int BS = TILE_M <= 64 ? 4 : (TILE_M <= 128 ? 2 : 1);
+  static constexpr int BOX_BYTES = TILE_M * BK * 2;
+  static constexpr int ACT_BYTES = BS * BOX_BYTES;
+  static constexpr int T_STAGE = BS * T_COLS;
+  static constexpr int STAGES = TILE_M <= 64 ? 3 : (TILE_M <= 128 ? 4 : 5);
+  static constexpr int ACC_COL = TILE_M <= 128 ? STAGES * T_STAGE : 256;
+  static constexpr int W_SLOT = BS * (WBLOCK_BYTES + 512);  // + up to two groups of scales a block
   static constexpr int ACT_OFF = 0;
   static constexpr int W_OFF = ACT_OFF + STAGES * ACT_BYTES;
   static constexpr int SPACE = 232448 - 1024 - W_OFF - kTableInts * 4 - 1024;
   static constexpr int W_FIT = SPACE / W_SLOT;
-  static constexpr int W_STAGES = W_FIT > 36 ? 36 : W_FIT;
+  static constexpr int W_STAGES = W_FIT > 32 / BS ? 32 / BS : W_FIT;
   static constexpr int TABLE_OFF = W_OFF + W_STAGES * W_SLOT;
   static constexpr int BAR_OFF = (TABLE_OFF + kTableInts * 4 + 15) / 16 * 16;
   static constexpr int NUM_BARS = 2 * STAGES + 2 * W_STAGES + 2 * ACC + 1;
   static constexpr int MISC_OFF = BAR_OFF + NUM_BARS * 8;
   static constexpr int DYN_BYTES = MISC_OFF + 32 + 1024;
   static_assert(COLS % 16 == 0, "the epilogue works in 16-column chunks");
-  static_assert(ACT_BYTES % 1024 == 0, "activation stages keep 1024-byte alignment");
-  static_assert(STAGES * T_COLS <= ACC_COL && ACC_COL + ACC * TILE_M <= TMEM_COLS, "TMEM");
+  static_assert(BOX_BYTES % 1024 == 0, "activation stages keep 1024-byte alignment");
+  static_assert(STAGES * T_STAGE <= ACC_COL && ACC_COL + ACC * TILE_M <= TMEM_COLS, "TMEM");
   static_assert(DYN_BYTES <= 232448, "shared memory");
-  static_assert(W_STAGES >= 8, "packed weights in flight");
+  static_assert(W_STAGES * BS >= 8, "packed weights in flight");
 };
 
+// K is walked in units of a stage (BS blocks; the last one may be shorter).
 // The cost of a split tail against a whole one, in 64-k blocks of a CTA's
 // time: publishing a partial tile, the ticket and the last arriver's sums.
 template <int TILE_M>
@@ -92,16 +100,16 @@ constexpr int split_overhead_blocks() {
 constexpr int kMinChunkBlocks = 8;
 constexpr int kMaxShares = 8;  // shares per tail tile on average
 
-__host__ __device__ inline Sched make_sched(int tiles, int kblocks, int units, bool split,
+__host__ __device__ inline Sched make_sched(int tiles, int kunits, int bs, int ctas, bool split,
                                             int overhead) {
   Sched s{tiles, 0, 0};
-  const int rem = tiles % units;
+  const int rem = tiles % ctas;
   if (!split || rem == 0) return s;
-  const int run = rem * kblocks;
-  int chunks = run / kMinChunkBlocks;
-  if (chunks > units) chunks = units;
+  const int run = rem * kunits;
+  int chunks = run * bs / kMinChunkBlocks;
+  if (chunks > ctas) chunks = ctas;
   if (chunks > rem * kMaxShares) chunks = rem * kMaxShares;
-  if (chunks <= rem || (run + chunks - 1) / chunks + overhead >= kblocks) return s;
+  if (chunks <= rem || ((run + chunks - 1) / chunks) * bs + overhead >= kunits * bs) return s;
   s.full_tiles = tiles - rem;
   s.tail_tiles = rem;
   s.chunks = chunks;
@@ -111,52 +119,60 @@ __host__ __device__ inline Sched make_sched(int tiles, int kblocks, int units, b
 // One CTA's share of a launch's work, and its items in order.
 struct Walk {
   Sched s;
-  int b, units, kblocks, num_n;
+  int b, ctas, kunits, num_n;
   int whole;   // whole tiles of this CTA
-  int c0, c1;  // its run of the tail's blocks
+  int c0, c1;  // its run of the tail's units
   const int* table;  // first m-tile of each expert (shared memory), [E + 1]
   const int* offsets;
-  int E, M, tile_m;
+  int E, M, num_m;   // num_m: m-tiles of the one weight (dense)
 
   __device__ __forceinline__ void start() {
-    whole = b < s.full_tiles ? (s.full_tiles - 1 - b) / units + 1 : 0;
+    whole = b < s.full_tiles ? (s.full_tiles - 1 - b) / ctas + 1 : 0;
     c0 = c1 = 0;
     if (b < s.chunks) {
-      const int run = s.tail_tiles * kblocks;
+      const int run = s.tail_tiles * kunits;
       c0 = static_cast<int>(static_cast<long long>(b) * run / s.chunks);
       c1 = static_cast<int>(static_cast<long long>(b + 1) * run / s.chunks);
     }
   }
-  __device__ __forceinline__ int blocks() const { return whole * kblocks + (c1 - c0); }
+  __device__ __forceinline__ int units() const { return whole * kunits + (c1 - c0); }
 };
 
 struct Item {
-  int e, nt, kb0, kb1;
+  int e, nt, u0, u1;  // units [u0, u1)
   int row0, rows;  // first row of C (sorted row), rows of this tile (1 .. TILE_M)
   int rem;         // tail tile, or -1: a whole tile
   int slot, base_slot, nparts;
 };
 
+// The units [u0, u1) of this CTA's j-th item (item_at without its place).
+__device__ __forceinline__ bool span_at(const Walk& w, int j, int& u0, int& u1) {
+  u0 = 0;
+  u1 = w.kunits;
+  if (j < w.whole) return true;
+  if (w.c1 <= w.c0) return false;
+  const int t = w.c0 / w.kunits + (j - w.whole);
+  if (t > (w.c1 - 1) / w.kunits) return false;
+  u0 = max(w.c0 - t * w.kunits, 0);
+  u1 = min(w.c1 - t * w.kunits, w.kunits);
+  return true;
+}
+
 template <int TILE_M>
 __device__ __forceinline__ bool item_at(const Walk& w, int j, Item& r) {
   int tile;
-  r.kb0 = 0;
-  r.kb1 = w.kblocks;
+  if (!span_at(w, j, r.u0, r.u1)) return false;
   r.rem = -1;
   if (j < w.whole) {
-    tile = w.b + j * w.units;
+    tile = w.b + j * w.ctas;
   } else {
-    if (w.c1 <= w.c0) return false;
-    const int t = w.c0 / w.kblocks + (j - w.whole);
-    if (t > (w.c1 - 1) / w.kblocks) return false;
-    r.kb0 = max(w.c0 - t * w.kblocks, 0);
-    r.kb1 = min(w.c1 - t * w.kblocks, w.kblocks);
+    const int t = w.c0 / w.kunits + (j - w.whole);
     tile = w.s.full_tiles + t;
-    // the shares of tile t: owner(v) is the last share starting at or before block v
-    const long long run = static_cast<long long>(w.s.tail_tiles) * w.kblocks;
-    const long long v0 = static_cast<long long>(t) * w.kblocks;
+    // the shares of tile t: owner(v) is the last share starting at or before unit v
+    const long long run = static_cast<long long>(w.s.tail_tiles) * w.kunits;
+    const long long v0 = static_cast<long long>(t) * w.kunits;
     const int p0 = static_cast<int>(((v0 + 1) * w.s.chunks - 1) / run);
-    const int p1 = static_cast<int>(((v0 + w.kblocks) * w.s.chunks - 1) / run);
+    const int p1 = static_cast<int>(((v0 + w.kunits) * w.s.chunks - 1) / run);
     if (p0 != p1) {
       r.rem = t;
       r.slot = t + w.b;  // unique: tiles and shares both only advance
@@ -174,7 +190,8 @@ __device__ __forceinline__ bool item_at(const Walk& w, int j, Item& r) {
     }
     e = lo;
   }
-  const int first = w.table[e], num_m = w.table[e + 1] - first;
+  const int first = w.offsets ? w.table[e] : 0;
+  const int num_m = w.offsets ? w.table[e + 1] - first : w.num_m;
   int mt;
   tile_coords(tile - first * w.num_n, num_m, w.num_n, mt, r.nt);
   r.e = e;
@@ -284,15 +301,16 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
   volatile uint32_t* ticket_slot = reinterpret_cast<volatile uint32_t*>(smem + L::MISC_OFF + 8);
   volatile int* never = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 12);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = static_cast<int>(uniform(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
   const int kblocks = a.K / BK;
+  const int kunits = (kblocks + L::BS - 1) / L::BS;
   const int groups = a.K / GROUP;
   const int num_n = a.N / TILE_N;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(full(i), 1 + 4 * 32);  // the activation copy and 128 dequant threads
+      mbar_init(full(i), 1 + 4);  // the activation copy and four dequant warps
       mbar_init(empty(i), 1);
     }
     for (int i = 0; i < W_STAGES; ++i) {
@@ -301,7 +319,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     }
     for (int i = 0; i < ACC; ++i) {
       mbar_init(dfull(i), 1);
-      mbar_init(dempty(i), L::EPI_WARPS * 32);
+      mbar_init(dempty(i), L::EPI_WARPS);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -314,67 +332,80 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
-  // Only set-up precedes the wait for the kernel before this one (programmatic
-  // dependent launch): offsets, rows, A, C and the workspace come after it.
-  grid_dependency_wait();
-  if (threadIdx.x == 0) launch_dependents();
-  // m-tiles before each expert
-  int mine = 0;
-  if (a.offsets) {
-    const int e = threadIdx.x;
-    if (e < a.E) {
-      const int lo = min(max(a.offsets[e], 0), a.M);
-      const int hi = min(max(a.offsets[e + 1], lo), a.M);
-      mine = (hi - lo + TILE_M - 1) / TILE_M;
-    }
-    int sum = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += o;
-    }
-    mine = sum;  // inclusive, within the warp
-    if (lane == 31) table[kMaxExperts + 1 + warp] = sum;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  if (a.offsets) {
-    int before = 0;
-    for (int i = 0; i < warp; ++i) before += table[kMaxExperts + 1 + i];
-    if (threadIdx.x < a.E) table[threadIdx.x + 1] = before + mine;
-    if (threadIdx.x == 0) table[0] = 0;
-  } else if (threadIdx.x == 0) {
-    table[0] = 0;
-    table[1] = (a.M + TILE_M - 1) / TILE_M;
-  }
-  __syncthreads();
+  const uint32_t tmem_base = uniform(*tmem_slot);
 
   Walk walk;
-  walk.units = gridDim.x;
+  walk.ctas = gridDim.x;
   walk.b = blockIdx.x;
-  walk.kblocks = kblocks;
+  walk.kunits = kunits;
   walk.num_n = num_n;
   walk.table = table;
   walk.offsets = a.offsets;
   walk.E = a.offsets ? a.E : 1;
   walk.M = a.M;
-  walk.s = make_sched(table[walk.E] * num_n, kblocks, gridDim.x, a.tickets != nullptr,
-                      split_overhead_blocks<TILE_M>());
-  walk.start();
+  walk.num_m = (a.M + TILE_M - 1) / TILE_M;
+  // Launched as a programmatic dependent, this CTA may come this far while the
+  // kernel before it still runs; A, C, the weights, the routing and the
+  // workspace are touched only after the wait. Before it the dense product,
+  // whose first weights are known, warms L2 with one ring of them (a prefetch
+  // cannot return stale data); the experts' tiles follow from the routing.
+  if (!a.offsets) {
+    walk.s = make_sched(walk.num_m * num_n, kunits, L::BS, gridDim.x, a.tickets != nullptr,
+                        split_overhead_blocks<TILE_M>());
+    walk.start();
+    if (warp == 2) {
+      Item w;
+      if (item_at<TILE_M>(walk, 0, w) && lane == 0) {
+        const int kb = w.u0 * L::BS;
+        const int nb = min(min(w.u1 * L::BS, kblocks) - kb, W_STAGES * L::BS);
+        const uint8_t* src = a.tiles + (static_cast<size_t>(w.nt) * kblocks + kb) * WBLOCK_BYTES;
+        for (int b = 0; b < nb; b += 16)
+          bulk_prefetch_l2(src + b * WBLOCK_BYTES, min(16, nb - b) * WBLOCK_BYTES);
+      }
+      __syncwarp();
+    }
+  }
+  grid_dependency_wait();
+  if (threadIdx.x == 0) launch_dependents();
+  if (a.offsets) {
+    // m-tiles before each expert
+    const int e = threadIdx.x;
+    int sum = 0;
+    if (e < a.E) {
+      const int lo = min(max(a.offsets[e], 0), a.M);
+      const int hi = min(max(a.offsets[e + 1], lo), a.M);
+      sum = (hi - lo + TILE_M - 1) / TILE_M;
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 31) table[kMaxExperts + 1 + warp] = sum;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) sum += table[kMaxExperts + 1 + i];
+    if (e < a.E) table[e + 1] = sum;
+    if (e == 0) table[0] = 0;
+    __syncthreads();
+    walk.s = make_sched(table[a.E] * num_n, kunits, L::BS, gridDim.x, a.tickets != nullptr,
+                        split_overhead_blocks<TILE_M>());
+    walk.start();
+  }
 
   if (warp == 0) {
     // ------------------------------------------------- activation producer
     // Gathered rows: lane l fetches rows 4 l .. 4 l + 3 of the tile (and 128
-    // further where the tile has them); rows past the tile's last repeat its
-    // last one and are never stored.
-    constexpr int GATHERS = TILE_M / 4;
-    constexpr int PER_LANE = (GATHERS + 31) / 32;
-    uint32_t it = 0;
+    // further where the tile has them) while there are any; the last fetch may
+    // repeat the tile's last row. Rows that are not fetched keep what the
+    // stage held: each belongs to one accumulator column, which is not stored.
+    constexpr int PER_LANE = (TILE_M / 4 + 31) / 32;
+    uint32_t it = 0, s = 0, ph = 0;
     bool ok = true;
     Item w;
-    for (int j = 0; ok && item_at<TILE_M>(walk, j, w); ++j) {
+    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
       int src[PER_LANE][4];
       if (a.rows) {
 #pragma unroll
@@ -385,23 +416,33 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
             src[q][i] = a.rows[w.row0 + r] / a.row_div;
           }
       }
-      for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-        const int s = it % STAGES;
-        const uint32_t ph = (it / STAGES) & 1u;
-        ok = mbar_wait(empty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
-        ok = __all_sync(0xffffffffu, ok);
+      const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
+      const int row0 = static_cast<int>(uniform(w.row0));
+      const int quads = static_cast<int>(uniform((w.rows + 3) / 4));
+      for (int u = u0; u < u1; ++u) {
+        ok = mbar_wait_warp(empty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(full(s), L::ACT_BYTES);
-        __syncwarp();
+        const int nb = min(L::BS, kblocks - u * L::BS);
         const uint32_t dst = act_base + s * L::ACT_BYTES;
+        if (elect_one()) {
+          // a box past the last block (the unit's second, of an odd K / 64)
+          // reads zeros and counts its bytes like any other
+          mbar_arrive_expect_tx(full(s), a.rows ? nb * quads * 512 : L::ACT_BYTES);
+          if (!a.rows) tma_load_3d(dst, &act_map, full(s), 0, row0, u * L::BS);
+        }
         if (a.rows) {
+          __syncwarp();
+          for (int b = 0; b < nb; ++b)
 #pragma unroll
-          for (int q = 0; q < PER_LANE; ++q)
-            if (GATHERS >= 32 || lane < GATHERS)
-              tma_gather4(dst + (lane + 32 * q) * 512, &act_map, full(s), kb * BK, src[q][0],
-                          src[q][1], src[q][2], src[q][3]);
-        } else if (lane == 0) {
-          tma_load_2d(dst, &act_map, full(s), kb * BK, w.row0);
+            for (int q = 0; q < PER_LANE; ++q)
+              if (lane + 32 * q < quads)
+                tma_gather4(dst + b * L::BOX_BYTES + (lane + 32 * q) * 512, &act_map, full(s),
+                            (u * L::BS + b) * BK, src[q][0], src[q][1], src[q][2], src[q][3]);
+        }
+        ++it;
+        if (++s == static_cast<uint32_t>(STAGES)) {
+          s = 0;
+          ph ^= 1u;
         }
       }
     }
@@ -411,151 +452,197 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     }
   } else if (warp == 2) {
     // ----------------------------------------------------- weight producer
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      Item w;
-      for (int j = 0; ok && item_at<TILE_M>(walk, j, w); ++j) {
-        const size_t col = static_cast<size_t>(w.e) * num_n + w.nt;  // 128-column run
-        const uint8_t* wblk = a.tiles + col * kblocks * WBLOCK_BYTES;
-        const __half* sblk = a.scales + col * groups * TILE_N;
-        for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-          const int s = it % W_STAGES;
-          const uint32_t ph = (it / W_STAGES) & 1u;
-          if (!mbar_wait(wempty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns)) {
-            ok = false;
-            break;
-          }
-          const int g0 = GROUP == 32 ? 2 * kb : (GROUP == 64 ? kb : kb >> 1);
-          constexpr uint32_t sbytes = GROUP == 32 ? 512 : 256;
-          mbar_arrive_expect_tx(wfull(s), WBLOCK_BYTES + sbytes);
-          bulk_load(w_base + s * W_SLOT, wblk + static_cast<size_t>(kb) * WBLOCK_BYTES,
-                    WBLOCK_BYTES, wfull(s));
-          bulk_load(w_base + s * W_SLOT + WBLOCK_BYTES, sblk + static_cast<size_t>(g0) * TILE_N,
-                    sbytes, wfull(s));
+    uint32_t s = 0, ph = 0, issued = 0;
+    bool ok = true;
+    Item w;
+    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
+      const size_t col = uniform(static_cast<uint32_t>(w.e * num_n + w.nt));  // 128-column run
+      const uint8_t* wsrc = a.tiles + col * kblocks * WBLOCK_BYTES;
+      const __half* ssrc = a.scales + col * groups * TILE_N;
+      const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
+      for (int u = u0; u < u1; ++u) {
+        ok = mbar_wait_warp(wempty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
+        if (!ok) break;
+        if (elect_one()) {
+          const int kb = u * L::BS, nb = min(L::BS, kblocks - kb);
+          const int g0 = kb * BK / GROUP, g1 = ((kb + nb) * BK + GROUP - 1) / GROUP;
+          const uint32_t dst = w_base + s * L::W_SLOT;
+          mbar_arrive_expect_tx(wfull(s), nb * WBLOCK_BYTES + (g1 - g0) * 256);
+          bulk_load(dst, wsrc + static_cast<size_t>(kb) * WBLOCK_BYTES, nb * WBLOCK_BYTES,
+                    wfull(s));
+          bulk_load(dst + L::BS * WBLOCK_BYTES, ssrc + static_cast<size_t>(g0) * TILE_N,
+                    (g1 - g0) * 256, wfull(s));
+        }
+        ++issued;
+        if (++s == static_cast<uint32_t>(W_STAGES)) {
+          s = 0;
+          ph ^= 1u;
         }
       }
-      if (!ok) {
-        for (uint32_t i = it > W_STAGES ? it - W_STAGES : 0; i < it; ++i)
-          mbar_wait(wfull(i % W_STAGES), (i / W_STAGES) & 1u, never, nullptr, 100000000ull);
-      }
+    }
+    if (!ok && lane == 0) {  // let every copy already issued land
+      for (uint32_t i = issued > W_STAGES ? issued - W_STAGES : 0; i < issued; ++i)
+        mbar_wait(wfull(i % W_STAGES), (i / W_STAGES) & 1u, never, nullptr, 100000000ull);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issue
-    if (lane == 0) {
-      constexpr uint32_t IDESC = idesc_f16_f32(TILE_N, TILE_M);
-      const uint64_t b_desc0 = smem_desc_sw128(act_base);
-      uint32_t s = 0, ph = 0;
-      uint32_t uses[2] = {0, 0};  // segments committed per accumulator
-      int acc = 0;
-      bool ok = true;
-      Item w;
-      for (int j = 0; ok && item_at<TILE_M>(walk, j, w); ++j) {
-        uint32_t used = acc == 0 ? uses[0] : uses[1];
-        if (!mbar_wait_lean(dempty(acc), (used & 1u) ^ 1u, abort_flag, a.status,
-                            a.wait_limit_ns)) {
-          ok = false;
+    // Unrolled over the ring's stages, so that every operand is a constant
+    // away from a loop-invariant (uniform) register: computed from a stage
+    // variable, operands alone took half of the time between two MMAs.
+    constexpr uint32_t IDESC = idesc_f16_f32(TILE_N, TILE_M);
+    const uint64_t b_desc = smem_desc_sw128(act_base);
+    uint32_t used[2] = {0, 0};  // segments committed per accumulator
+    uint32_t ph = 0;
+    int acc = ACC - 1, j = 0;
+    int u = 0, u1 = 0, end = 0;  // next unit, past the item's last, past the segment's
+    bool fresh = true;           // the item's first MMA starts the sum
+    // Ends a segment and starts the next one, of this item or of the next;
+    // false past the last (or after a failed wait).
+    auto next_segment = [&]() -> bool {
+      if (u == u1) {
+        int first, last;
+        if (!__any_sync(0xffffffffu, span_at(walk, j++, first, last))) return false;
+        u = static_cast<int>(uniform(first));
+        u1 = static_cast<int>(uniform(last));
+        if (ACC == 2) acc ^= 1;
+        fresh = true;
+      }
+      end = min(u1, u + kPromoteBlocks / L::BS);
+      const uint32_t n = acc == 0 ? used[0] : used[1];
+      if (acc == 0) ++used[0]; else ++used[1];
+      if (!mbar_wait_warp(dempty(acc), (n & 1u) ^ 1u, abort_flag, a.status, a.wait_limit_ns))
+        return false;
+      tc_fence_after();
+      return true;
+    };
+    bool more = next_segment();
+    while (more) {
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) {
+        if (!mbar_wait_warp(full(s), ph, abort_flag, a.status, a.wait_limit_ns)) {
+          more = false;
           break;
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
-        int left = kPromoteBlocks;
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (left == 0) {
-            // segment boundary: the epilogue promotes, then the MMAs go on
-            tc_commit(dfull(acc));
-            ++used;
-            if (!mbar_wait_lean(dempty(acc), (used & 1u) ^ 1u, abort_flag, a.status,
-                                a.wait_limit_ns)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            left = kPromoteBlocks;
-          }
-          --left;
-          if (!mbar_wait_lean(full(s), ph, abort_flag, a.status, a.wait_limit_ns)) {
-            ok = false;
+#pragma unroll
+        for (int b = 0; b < L::BS; ++b) {
+          if (b > 0 && u * L::BS + b >= kblocks) break;
+          mma_f16_ts_block(d_tmem, tmem_base + s * L::T_STAGE + b * T_COLS,
+                           b_desc + ((s * L::ACT_BYTES + b * L::BOX_BYTES) >> 4), IDESC,
+                           b == 0 && fresh ? 0u : 1u);
+        }
+        fresh = false;
+        if (elect_one()) tc_commit(empty(s));
+        if (++u == end) {
+          if (elect_one()) tc_commit(dfull(acc));
+          if (!next_segment()) {
+            more = false;
             break;
           }
-          tc_fence_after();
-          const uint64_t b_desc = b_desc0 + ((s * L::ACT_BYTES) >> 4);
-          const uint32_t a_tmem = tmem_base + s * T_COLS;
-          const uint32_t first = kb != w.kb0;
-#pragma unroll
-          for (int k16 = 0; k16 < BK / 16; ++k16)
-            mma_f16_ts(d_tmem, a_tmem + 8 * k16, b_desc + 2 * k16, IDESC, k16 == 0 ? first : 1u);
-          tc_commit(empty(s));
-          if (++s == static_cast<uint32_t>(STAGES)) {
-            s = 0;
-            ph ^= 1u;
-          }
         }
-        if (!ok) break;
-        tc_commit(dfull(acc));
-        ++used;
-        if (acc == 0) uses[0] = used; else uses[1] = used;
-        if (ACC == 2) acc ^= 1;
       }
-      tc_commit(drain_bar);  // TMEM is freed only after every MMA completed
-      mbar_wait(drain_bar, 0, never, nullptr, 100000000ull);
+      ph ^= 1u;
     }
+    if (elect_one()) tc_commit(drain_bar);  // TMEM is freed only after every MMA completed
+    mbar_wait_warp(drain_bar, 0, never, nullptr, 100000000ull);
   } else if (warp < L::FIRST_EPI_WARP) {
     // ---------------------------------------------------------------- dequant
     const uint32_t dgroup = static_cast<uint32_t>(warp - FIRST_DEQ_WARP) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // weight column inside the tile
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t total = static_cast<uint32_t>(walk.blocks());
-    for (uint32_t it = dgroup; it < total; it += L::DEQ) {
-      const int s = it % W_STAGES;
-      const int ts = it % STAGES;
-      const bool landed = mbar_wait(wfull(s), (it / W_STAGES) & 1u, abort_flag, a.status,
-                                    a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, landed)) break;  // a warp leaves as a whole
-      const uint32_t wsrc = w_base + s * W_SLOT + row * 16;
-      uint4 c0, c1;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(c0.x), "=r"(c0.y), "=r"(c0.z), "=r"(c0.w)
-                   : "r"(wsrc));
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(c1.x), "=r"(c1.y), "=r"(c1.z), "=r"(c1.w)
-                   : "r"(wsrc + 2048));
-      uint16_t sb0, sb1;
-      const uint32_t ssrc = w_base + s * W_SLOT + WBLOCK_BYTES + row * 2;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb0) : "r"(ssrc));
-      if (GROUP == 32)
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb1) : "r"(ssrc + TILE_N * 2));
-      else
-        sb1 = sb0;
-      const uint32_t s0 = half_bits_x2(sb0), s1 = half_bits_x2(sb1);
-      uint32_t r[32];
-      const uint32_t wv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    int ws = 0, ts = 0;
+    uint32_t wph = 0, tph = 0, turn = 0;
+    bool ok = true;
+    Item w;
+    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
+      const int u1 = static_cast<int>(uniform(w.u1));
+      for (int u = static_cast<int>(uniform(w.u0)); u < u1; ++u) {
+        if (turn == dgroup) {
+          ok = mbar_wait_warp(wfull(ws), wph, abort_flag, a.status, a.wait_limit_ns);
+          if (!ok) break;
+          const uint32_t slot = w_base + ws * L::W_SLOT;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t sc = i < 4 ? s0 : s1;
-        r[4 * i + 0] = decode_pair<0>(wv[i], sc);
-        r[4 * i + 1] = decode_pair<1>(wv[i], sc);
-        r[4 * i + 2] = decode_pair<2>(wv[i], sc);
-        r[4 * i + 3] = decode_pair<3>(wv[i], sc);
+          for (int b = 0; b < L::BS; ++b) {
+            if (L::BS > 1 && b > 0 && u * L::BS + b >= kblocks) break;
+            const uint32_t wsrc = slot + b * WBLOCK_BYTES + row * 16;
+            uint4 c0, c1;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(c0.x), "=r"(c0.y), "=r"(c0.z), "=r"(c0.w)
+                         : "r"(wsrc));
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(c1.x), "=r"(c1.y), "=r"(c1.z), "=r"(c1.w)
+                         : "r"(wsrc + 2048));
+            uint16_t sb0, sb1;
+            // the block's first scale group inside the unit (a group of 128
+            // holds both blocks of a unit)
+            constexpr int kGroups = GROUP == 32 ? 2 : 1;
+            const uint32_t ssrc = slot + L::BS * WBLOCK_BYTES +
+                                  (GROUP == 128 ? b / 2 : b * kGroups) * (TILE_N * 2) + row * 2;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb0) : "r"(ssrc));
+            if (GROUP == 32)
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb1) : "r"(ssrc + TILE_N * 2));
+            else
+              sb1 = sb0;
+            const uint32_t s0 = half_bits_x2(sb0), s1 = half_bits_x2(sb1);
+            uint32_t r[32];
+            const uint32_t wv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            const float f0 = fabsf(__half2float(__ushort_as_half(sb0)));
+            const float f1 = fabsf(__half2float(__ushort_as_half(sb1)));
+            if (__all_sync(0xffffffffu, f0 < kFastScale && f1 < kFastScale)) {
+              const __half2 k1024 = __float2half2_rn(1024.0f), km8 = __float2half2_rn(-8.0f);
+              const __half2 h0 = u32_as_half2(s0), h1 = u32_as_half2(s1);
+              const uint32_t up0 = half2_as_u32(__hmul2(__hmul2(h0, k1024), k1024));
+              const uint32_t up1 = half2_as_u32(__hmul2(__hmul2(h1, k1024), k1024));
+              const uint32_t m0 = half2_as_u32(__hmul2(h0, km8));
+              const uint32_t m1 = half2_as_u32(__hmul2(h1, km8));
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                decode_word(wv[i], i < 4 ? up0 : up1, i < 4 ? m0 : m1, &r[4 * i]);
+            } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t sc = i < 4 ? s0 : s1;
+              r[4 * i + 0] = decode_pair<0>(wv[i], sc);
+              r[4 * i + 1] = decode_pair<1>(wv[i], sc);
+              r[4 * i + 2] = decode_pair<2>(wv[i], sc);
+              r[4 * i + 3] = decode_pair<3>(wv[i], sc);
+            }
+            }
+            if (b == 0) {
+              ok = mbar_wait_warp(empty(ts), tph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            tmem_st_32x32b_x32(tmem_base + lane_addr + ts * L::T_STAGE + b * T_COLS, r);
+          }
+          if (!ok) break;
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(full(ts));
+            // The packed slot is given back only now: the TMEM store has
+            // consumed what was loaded from it. An arrival right after the
+            // loads can overtake them (they queue behind the epilogue's global
+            // stores, the arrival does not), and the next copy into the slot
+            // then overtakes the loads: one 64-k block of some columns was
+            // wrong in every second launch of M = 1024, N = 2048, K = 12288,
+            // where partial tiles are stored while the pipeline runs.
+            mbar_arrive(wempty(ws));
+          }
+        }
+        if (++turn == L::DEQ) turn = 0;
+        if (++ws == W_STAGES) {
+          ws = 0;
+          wph ^= 1u;
+        }
+        if (++ts == STAGES) {
+          ts = 0;
+          tph ^= 1u;
+        }
       }
-      const bool free = mbar_wait(empty(ts), ((it / STAGES) & 1u) ^ 1u, abort_flag, a.status,
-                                  a.wait_limit_ns);
-      if (!__all_sync(0xffffffffu, free)) break;
-      tc_fence_after();
-      tmem_st_32x32b_x32(tmem_base + lane_addr + ts * T_COLS, r);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(full(ts));
-      // The packed slot is given back only now: the TMEM store has consumed
-      // what was loaded from it. An arrival right after the loads can overtake
-      // them (they queue behind the epilogue's global stores, the arrival does
-      // not), and the next copy into the slot then overtakes the loads: one
-      // 64-k block of some columns was wrong in every second launch of
-      // M = 1024, N = 2048, K = 12288, where partial tiles are stored while
-      // the pipeline runs.
-      __syncwarp();
-      if (lane == 0) mbar_arrive(wempty(s));
     }
   } else {
     // --------------------------------------------------------------- epilogue
@@ -592,7 +679,8 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
                       ? __half2float(a.epilogue.bias[static_cast<size_t>(w.e) * a.N +
                                                      w.nt * TILE_N + row])
                       : 0.0f;
-      const int nseg = (w.kb1 - w.kb0 + kPromoteBlocks - 1) / kPromoteBlocks;
+      constexpr int kSeg = kPromoteBlocks / L::BS;  // units per segment
+      const int nseg = (w.u1 - w.u0 + kSeg - 1) / kSeg;
       uint32_t hb[COLS / 4];  // the running sum's high parts (e5m2 x4)
 #pragma unroll
       for (int q = 0; q < COLS / 4; ++q) hb[q] = 0u;
@@ -610,7 +698,8 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
           failed = true;
         }
         tc_fence_before();
-        mbar_arrive(dempty(acc));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dempty(acc));
       }
       // the shuffles of a gated pair need whole warps, so the outcome of the
       // wait is made the warp's
@@ -638,7 +727,8 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
             store16<GATED>(sink, m0 + c * 16, up, f);
           }
           tc_fence_before();
-          mbar_arrive(release_bar);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(release_bar);
         } else {
           // rounded to FP16 pairs in registers, the accumulator released,
           // then stored
@@ -657,7 +747,8 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
               hv[c * (KEEP / 2) + i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
           }
           tc_fence_before();
-          mbar_arrive(release_bar);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(release_bar);
           __half* const cp = static_cast<__half*>(a.C) + sink.c0;
 #pragma unroll
           for (int c = 0; c < COLS / 16; ++c)
@@ -690,7 +781,8 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
                                __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])));
         }
         tc_fence_before();
-        mbar_arrive(release_bar);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(release_bar);
         __threadfence();
       }
       if (!epi_bar_and(EPI_THREADS, ok)) {

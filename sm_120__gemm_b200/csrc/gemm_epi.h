@@ -38,6 +38,16 @@ struct Sched {
 
 // Activation rows per tile for `rows` rows per weight (16, 32, 64, 128, 256).
 int choose_tile(int rows);
+// Rows of a tile from which gathered activations are first copied into row
+// order by a kernel of their own (gather_rows) instead of four rows per copy
+// instruction inside the product.
+constexpr int kCopyRowsTile = 64;
+// 64-k blocks of the activation box of a tile height.
+int box_blocks(int tile_m);
+// out[p] = A[rows[p] / row_div] for p < offsets[E]; K halves a row.
+cudaError_t gather_rows(const __half* A, int a_rows, const int* offsets, const int* rows,
+                        int row_div, __half* out, int M, int E, int K, int sm_count,
+                        cudaStream_t stream);
 // Most tiles a launch can have (rows spread over E weights in the worst way).
 long tiles_bound(int tile_m, int M, int E, int N);
 // Workspace of the split tail for any number of tiles (0: nothing to split).

@@ -154,6 +154,48 @@ __device__ __forceinline__ bool mbar_wait_lean(uint32_t bar, uint32_t parity,
   return mbar_wait_slow(bar, parity, abort, status, limit_ns);
 }
 
+// True in one lane of a converged warp. A warp that issues tensor-core or copy
+// instructions from one elected lane inside warp-uniform control flow keeps
+// their operands in uniform registers; inside a lane == 0 branch the compiler
+// moves them there lane by lane (a 128 x 16 x 16 MMA: 31 against 52 cycles).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// A value that is the same in every lane of a converged warp, as one the
+// compiler knows to be: control flow that hangs on it stays warp-uniform.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return __reduce_max_sync(0xffffffffu, v);
+}
+
+// mbar_wait for a whole converged warp; the outcome is the same for every lane.
+// The polling loop is inline: around a call the compiler cannot keep the
+// operands of tensor-core instructions in uniform registers.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity,
+                                               volatile int* abort, int* status,
+                                               uint64_t limit_ns) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  while (!__all_sync(0xffffffffu, mbar_try_wait_sleep(bar, parity, 20000))) {
+    const bool late = global_timer_ns() - t0 > limit_ns;
+    if (__any_sync(0xffffffffu, late || *abort != 0)) {
+      if (late) {
+        *abort = 1;
+        if (status) atomicExch(status, kStatusTimeout);
+      }
+      return false;
+    }
+  }
+  return true;
+}
+
 // Named barrier 1 among `nthreads` threads (a subset of warps, e.g. those
 // that do not stream copies); `bar_and` also ANDs a per-thread predicate
 // across them.
@@ -442,6 +484,33 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// The four k16 steps of one 64-k block (operand A 8 TMEM columns and operand B
+// 32 bytes further per step), issued by one elected lane of a converged warp;
+// the first step starts the sum unless `accumulate`.
+__device__ __forceinline__ void mma_f16_ts_block(uint32_t d_tmem, uint32_t a_tmem,
+                                                 uint64_t b_desc, uint32_t idesc,
+                                                 uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred one, acc, yes;\n\t"
+      ".reg .b32 a1, a2, a3;\n\t"
+      ".reg .b64 b1, b2, b3;\n\t"
+      "elect.sync _|one, 0xffffffff;\n\t"
+      "setp.ne.b32 acc, %4, 0;\n\t"
+      "setp.eq.b32 yes, 0, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\t"
+      "add.u32 a2, %1, 16;\n\t"
+      "add.u32 a3, %1, 24;\n\t"
+      "add.u64 b1, %2, 2;\n\t"
+      "add.u64 b2, %2, 4;\n\t"
+      "add.u64 b3, %2, 6;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, acc;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, yes;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, yes;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, yes;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Shared-memory matrix descriptor for a K-major operand stored as rows of
 // 128 bytes with the 128-byte swizzle (8-row atoms 1024 bytes apart).
 __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
@@ -573,6 +642,26 @@ __device__ __forceinline__ uint32_t decode_pair(uint32_t word, uint32_t scale2) 
   const uint32_t biased = (x & 0x000F000Fu) ^ 0x64086408u;
   const __half2 q = __hsub2(u32_as_half2(biased), u32_as_half2(0x64086408u));
   return half2_as_u32(__hmul2(q, u32_as_half2(scale2)));
+}
+
+// The four pairs of a tile-layout word, as decode_pair gives them, in one
+// multiply-add per pair. A nibble XOR 8 is u = q + 8; at bits 4..7 of a half
+// (the other bits zero) it is the subnormal u 2^-20. fma(u 2^-20, s 2^20, -8 s)
+// has the exact value q s before its one rounding, so it is half(q * s) bit
+// for bit, as long as s 2^20 is finite and -8 s exact: |s| < kFastScale.
+// 11 instructions of the half-rate pipes a word, against 15 (which bounds the
+// kernel at 234 cycles a 64-k block, three warps per scheduler; this form 170).
+constexpr float kFastScale = 0.0624f;  // 65504 / 2^20 = 0.06247
+
+__device__ __forceinline__ void decode_word(uint32_t word, uint32_t scale_2p20, uint32_t minus_8s,
+                                            uint32_t* out) {
+  const uint32_t x[4] = {word << 4, word, word >> 4, word >> 8};
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t u = (x[p] & 0x00F000F0u) ^ 0x00800080u;
+    out[p] = half2_as_u32(
+        __hfma2(u32_as_half2(u), u32_as_half2(scale_2p20), u32_as_half2(minus_8s)));
+  }
 }
 
 __device__ __forceinline__ uint32_t half_bits_x2(uint16_t h) {
