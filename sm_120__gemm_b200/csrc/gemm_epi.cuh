@@ -75,7 +75,7 @@ struct Cfg {
   static constexpr int W_SLOT = BS * (WBLOCK_BYTES + 512);  // + up to two groups of scales a block
   static constexpr int ACT_OFF = 0;
   static constexpr int W_OFF = ACT_OFF + STAGES * ACT_BYTES;
-  static constexpr int SPACE = 232448 - 1024 - W_OFF - kTableInts * 4 - 1024;
+  static constexpr int SPACE = 232448 - 1024 - 1024 - W_OFF - kTableInts * 4 - 1024;
   static constexpr int W_FIT = SPACE / W_SLOT;
   static constexpr int W_STAGES = W_FIT > 32 / BS ? 32 / BS : W_FIT;
   static constexpr int TABLE_OFF = W_OFF + W_STAGES * W_SLOT;
@@ -87,6 +87,10 @@ struct Cfg {
   static_assert(BOX_BYTES % 1024 == 0, "activation stages keep 1024-byte alignment");
   static_assert(STAGES * T_STAGE <= ACC_COL && ACC_COL + ACC * TILE_M <= TMEM_COLS, "TMEM");
   static_assert(DYN_BYTES <= 232448, "shared memory");
+  // A group that stored unit i knows that the MMAs of unit i - STAGES are done;
+  // its next unit waits, by parity, for those of unit i + DEQ - STAGES, which
+  // is the right phase only if the one two phases before it is known to be over.
+  static_assert(DEQ <= STAGES && DEQ <= W_STAGES, "phases that parity can tell apart");
   static_assert(W_STAGES * BS >= 8, "packed weights in flight");
 };
 
@@ -486,63 +490,53 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issue
-    // Unrolled over the ring's stages, so that every operand is a constant
-    // away from a loop-invariant (uniform) register: computed from a stage
-    // variable, operands alone took half of the time between two MMAs.
-    constexpr uint32_t IDESC = idesc_f16_f32(TILE_N, TILE_M);
-    const uint64_t b_desc = smem_desc_sw128(act_base);
+    // Every loop bound is warp-uniform (see elect_one, uniform). A tile's MMAs
+    // are as wide as its rows (rounded up to 16); wider ones would only take
+    // longer.
+    const uint64_t b_desc0 = smem_desc_sw128(act_base);
+    uint32_t s = 0, ph = 0;
     uint32_t used[2] = {0, 0};  // segments committed per accumulator
-    uint32_t ph = 0;
-    int acc = ACC - 1, j = 0;
-    int u = 0, u1 = 0, end = 0;  // next unit, past the item's last, past the segment's
-    bool fresh = true;           // the item's first MMA starts the sum
-    // Ends a segment and starts the next one, of this item or of the next;
-    // false past the last (or after a failed wait).
-    auto next_segment = [&]() -> bool {
-      if (u == u1) {
-        int first, last;
-        if (!__any_sync(0xffffffffu, span_at(walk, j++, first, last))) return false;
-        u = static_cast<int>(uniform(first));
-        u1 = static_cast<int>(uniform(last));
-        if (ACC == 2) acc ^= 1;
-        fresh = true;
-      }
-      end = min(u1, u + kPromoteBlocks / L::BS);
-      const uint32_t n = acc == 0 ? used[0] : used[1];
-      if (acc == 0) ++used[0]; else ++used[1];
-      if (!mbar_wait_warp(dempty(acc), (n & 1u) ^ 1u, abort_flag, a.status, a.wait_limit_ns))
-        return false;
-      tc_fence_after();
-      return true;
-    };
-    bool more = next_segment();
-    while (more) {
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s) {
-        if (!mbar_wait_warp(full(s), ph, abort_flag, a.status, a.wait_limit_ns)) {
-          more = false;
-          break;
-        }
+    int acc = 0;
+    bool ok = true;
+    Item w;
+    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
+      const int u1 = static_cast<int>(uniform(w.u1));
+      int u = static_cast<int>(uniform(w.u0));
+      const uint32_t idesc = idesc_f16_f32(TILE_N, static_cast<int>(uniform((w.rows + 15) & ~15)));
+      const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
+      uint32_t accumulate = 0;  // the item's first MMA starts the sum
+      while (true) {
+        // one segment of at most kPromoteBlocks blocks, once the accumulator
+        // is free: the last item drained it, or the epilogue promoted it
+        const uint32_t n = acc == 0 ? used[0]++ : used[1]++;
+        ok = mbar_wait_warp(dempty(acc), (n & 1u) ^ 1u, abort_flag, a.status, a.wait_limit_ns);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
+        const int end = min(u1, u + kPromoteBlocks / L::BS);
+        for (; u < end; ++u) {
+          ok = mbar_wait_warp(full(s), ph, abort_flag, a.status, a.wait_limit_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t b_desc = b_desc0 + ((s * L::ACT_BYTES) >> 4);
+          const uint32_t a_tmem = tmem_base + s * L::T_STAGE;
 #pragma unroll
-        for (int b = 0; b < L::BS; ++b) {
-          if (b > 0 && u * L::BS + b >= kblocks) break;
-          mma_f16_ts_block(d_tmem, tmem_base + s * L::T_STAGE + b * T_COLS,
-                           b_desc + ((s * L::ACT_BYTES + b * L::BOX_BYTES) >> 4), IDESC,
-                           b == 0 && fresh ? 0u : 1u);
-        }
-        fresh = false;
-        if (elect_one()) tc_commit(empty(s));
-        if (++u == end) {
-          if (elect_one()) tc_commit(dfull(acc));
-          if (!next_segment()) {
-            more = false;
-            break;
+          for (int b = 0; b < L::BS; ++b) {
+            if (b > 0 && u * L::BS + b >= kblocks) break;
+            mma_f16_ts_block(d_tmem, a_tmem + b * T_COLS, b_desc + ((b * L::BOX_BYTES) >> 4),
+                             idesc, accumulate);
+            accumulate = 1;
+          }
+          if (elect_one()) tc_commit(empty(s));
+          if (++s == static_cast<uint32_t>(STAGES)) {
+            s = 0;
+            ph ^= 1u;
           }
         }
+        if (!ok) break;
+        if (elect_one()) tc_commit(dfull(acc));
+        if (u == u1) break;
       }
-      ph ^= 1u;
+      if (ACC == 2) acc ^= 1;
     }
     if (elect_one()) tc_commit(drain_bar);  // TMEM is freed only after every MMA completed
     mbar_wait_warp(drain_bar, 0, never, nullptr, 100000000ull);
@@ -552,6 +546,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // weight column inside the tile
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const NibbleMask nibble;
     int ws = 0, ts = 0;
     uint32_t wph = 0, tph = 0, turn = 0;
     bool ok = true;
@@ -588,27 +583,21 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
             const uint32_t s0 = half_bits_x2(sb0), s1 = half_bits_x2(sb1);
             uint32_t r[32];
             const uint32_t wv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-            const float f0 = fabsf(__half2float(__ushort_as_half(sb0)));
-            const float f1 = fabsf(__half2float(__ushort_as_half(sb1)));
-            if (__all_sync(0xffffffffu, f0 < kFastScale && f1 < kFastScale)) {
-              const __half2 k1024 = __float2half2_rn(1024.0f), km8 = __float2half2_rn(-8.0f);
-              const __half2 h0 = u32_as_half2(s0), h1 = u32_as_half2(s1);
-              const uint32_t up0 = half2_as_u32(__hmul2(__hmul2(h0, k1024), k1024));
-              const uint32_t up1 = half2_as_u32(__hmul2(__hmul2(h1, k1024), k1024));
-              const uint32_t m0 = half2_as_u32(__hmul2(h0, km8));
-              const uint32_t m1 = half2_as_u32(__hmul2(h1, km8));
+            if (__all_sync(0xffffffffu,
+                           fast_scale(sb0) && (GROUP != 32 || fast_scale(sb1)))) {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                decode_word(wv[i], i < 4 ? up0 : up1, i < 4 ? m0 : m1, &r[4 * i]);
+                decode_word(wv[i], (i < 4 ? s0 : s1) + kTimes2p20,
+                            (i < 4 ? s0 : s1) + kTimesMinus8, nibble, &r[4 * i]);
             } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t sc = i < 4 ? s0 : s1;
-              r[4 * i + 0] = decode_pair<0>(wv[i], sc);
-              r[4 * i + 1] = decode_pair<1>(wv[i], sc);
-              r[4 * i + 2] = decode_pair<2>(wv[i], sc);
-              r[4 * i + 3] = decode_pair<3>(wv[i], sc);
-            }
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t sc = i < 4 ? s0 : s1;
+                r[4 * i + 0] = decode_pair<0>(wv[i], sc);
+                r[4 * i + 1] = decode_pair<1>(wv[i], sc);
+                r[4 * i + 2] = decode_pair<2>(wv[i], sc);
+                r[4 * i + 3] = decode_pair<3>(wv[i], sc);
+              }
             }
             if (b == 0) {
               ok = mbar_wait_warp(empty(ts), tph ^ 1u, abort_flag, a.status, a.wait_limit_ns);

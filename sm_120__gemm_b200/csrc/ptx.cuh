@@ -648,20 +648,39 @@ __device__ __forceinline__ uint32_t decode_pair(uint32_t word, uint32_t scale2) 
 // multiply-add per pair. A nibble XOR 8 is u = q + 8; at bits 4..7 of a half
 // (the other bits zero) it is the subnormal u 2^-20. fma(u 2^-20, s 2^20, -8 s)
 // has the exact value q s before its one rounding, so it is half(q * s) bit
-// for bit, as long as s 2^20 is finite and -8 s exact: |s| < kFastScale.
-// 11 instructions of the half-rate pipes a word, against 15 (which bounds the
-// kernel at 234 cycles a 64-k block, three warps per scheduler; this form 170).
-constexpr float kFastScale = 0.0624f;  // 65504 / 2^20 = 0.06247
+// for bit, as long as s 2^20 is finite and -8 s exact. For a normal s both are
+// additions to the exponent field, so fast_scale admits 2^-14 <= s < 2^-4
+// (0x0400 .. 0x2BFF; times 2^20 at most 0x7BFF, the largest half). 11
+// instructions of the half-rate pipes a word, against decode_pair's 15.
+__device__ __forceinline__ bool fast_scale(uint32_t scale_bits) {
+  return scale_bits - 0x0400u < 0x2C00u - 0x0400u;
+}
+constexpr uint32_t kTimes2p20 = 0x50005000u;   // + 20 on both exponents
+constexpr uint32_t kTimesMinus8 = 0x8C008C00u;  // + 3, and the sign
+
+// The mask of the nibble and the bit that turns q into u, kept in registers:
+// as two immediates the and-xor would become two instructions (K = 65536,
+// N = 18944, 16 rows: 146 us so, 121 us with registers).
+struct NibbleMask {
+  uint32_t keep, flip;
+  __device__ __forceinline__ NibbleMask() {
+    asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(keep));
+    asm volatile("mov.b32 %0, 0x00800080;" : "=r"(flip));
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+    uint32_t u;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(u) : "r"(x), "r"(keep), "r"(flip));
+    return u;
+  }
+};
 
 __device__ __forceinline__ void decode_word(uint32_t word, uint32_t scale_2p20, uint32_t minus_8s,
-                                            uint32_t* out) {
+                                            const NibbleMask& nibble, uint32_t* out) {
   const uint32_t x[4] = {word << 4, word, word >> 4, word >> 8};
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const uint32_t u = (x[p] & 0x00F000F0u) ^ 0x00800080u;
-    out[p] = half2_as_u32(
-        __hfma2(u32_as_half2(u), u32_as_half2(scale_2p20), u32_as_half2(minus_8s)));
-  }
+  for (int p = 0; p < 4; ++p)
+    out[p] = half2_as_u32(__hfma2(u32_as_half2(nibble(x[p])), u32_as_half2(scale_2p20),
+                                  u32_as_half2(minus_8s)));
 }
 
 __device__ __forceinline__ uint32_t half_bits_x2(uint16_t h) {

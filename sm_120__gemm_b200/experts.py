@@ -17,10 +17,10 @@ from typing import NamedTuple
 
 import torch
 
-from . import (ACTIVATIONS, GROUP_SCORES, SCORINGS, RouteOptions, experts_workspace_size,
-               launch_combine, launch_experts, launch_quantize_repack, launch_repack_scales_128,
-               launch_repack_umma, launch_route, route_workspace_size)
-from .launching import on, want, want_out, workspace
+from . import (ACTIVATIONS, GROUP_SCORES, SCORINGS, Epilogue, RouteOptions,
+               experts_workspace_size, launch_quantize_repack, launch_repack_scales_128,
+               launch_repack_umma, route_workspace_size)
+from .launching import on, run, size, want, want_out, workspace
 from .linear import interleave_gate_up
 
 
@@ -54,18 +54,19 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
             logits = logits.contiguous()
         if bias is not None:
             bias = want(bias, "bias", torch.float32, (E,), dev).contiguous()
-        pairs = T * top_k
-        # one allocation: ids, slots, rows, offsets (int32) and weights (float32)
-        buf = torch.empty(4 * pairs + E + 1, dtype=torch.int32, device=dev)
-        ids, weights, slots, rows, offsets = buf.split((pairs, pairs, pairs, pairs, E + 1))
-        r = Routing(ids.view(T, top_k), weights.view(torch.float32).view(T, top_k), offsets, rows,
-                    slots.view(T, top_k))
+        r = Routing(torch.empty(T, top_k, dtype=torch.int32, device=dev),
+                    torch.empty(T, top_k, dtype=torch.float32, device=dev),
+                    torch.empty(E + 1, dtype=torch.int32, device=dev),
+                    torch.empty(T * top_k, dtype=torch.int32, device=dev),
+                    torch.empty(T, top_k, dtype=torch.int32, device=dev))
         options = RouteOptions(SCORINGS[scoring], n_group, topk_group, GROUP_SCORES[group_score],
-                               bool(renormalize), scale)
-        need = route_workspace_size(T, E)  # for its counts; nothing is kept in it
+                               renormalize, scale)
+        need = size(route_workspace_size, dev, T, E)  # for its counts; nothing is kept in it
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        launch_route(logits, logits.dtype == torch.float32, logits.stride(0) if T > 1 else E, bias,
-                     T, E, top_k, options, r.ids, r.weights, r.offsets, r.rows, r.slots, ws)
+        run("i4g_route", dev, logits.data_ptr(), logits.dtype == torch.float32,
+            logits.stride(0) if T > 1 else E, 0 if bias is None else bias.data_ptr(), T, E, top_k,
+            options, r.ids.data_ptr(), r.weights.data_ptr(), r.offsets.data_ptr(),
+            r.rows.data_ptr(), r.slots.data_ptr(), 0 if ws is None else ws.data_ptr(), need)
     return r
 
 
@@ -90,7 +91,9 @@ def combine(y: torch.Tensor, routing: Routing, *, residual: torch.Tensor | None 
             residual = want(residual, "residual", torch.float16, (T, N), dev).contiguous()
         if out is None:
             out = torch.empty(T, N, dtype=torch.float16, device=dev)
-        launch_combine(y, y.shape[0], slots, weights, residual, out, T, top_k, N)
+        run("i4g_experts_combine", dev, y.data_ptr(), y.shape[0], slots.data_ptr(),
+            weights.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(), T,
+            top_k, N)
     return out
 
 
@@ -181,10 +184,13 @@ class QuantizedExperts:
                 bias = want(bias, "bias", torch.float16, (self.E, self.N), dev).contiguous()
             if out is None:
                 out = torch.empty(pairs, cols, dtype=dtype, device=dev)
-            ws = workspace(_experts_workspace(dev, pairs, self.E, self.N, self.K), dev)
-            launch_experts(a, rows_a, self.tiles, self.scales, out, routing.offsets,
-                           routing.rows if gather else None, top_k, pairs, self.E, self.N, self.K,
-                           self.group, bias, activation, gated, fp32_out, ws)
+            ws = workspace(size(experts_workspace_size, dev, pairs, self.E, self.N, self.K), dev)
+            e = Epilogue(0 if bias is None else bias.data_ptr(), 0, 0, ACTIVATIONS[activation],
+                         gated, fp32_out)
+            run("i4g_experts_gemm", dev, a.data_ptr(), rows_a, self.tiles.data_ptr(),
+                self.scales.data_ptr(), out.data_ptr(), routing.offsets.data_ptr(),
+                routing.rows.data_ptr() if gather else 0, top_k, pairs, self.E, self.N, self.K,
+                self.group, e, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
         return out
 
 
@@ -205,15 +211,3 @@ class ExpertMLP:
         y = self.down(h, routing, gather=False, stream=stream)
         return combine(y, routing, residual=residual, stream=stream)
 
-
-_sizes: dict = {}
-
-
-def _experts_workspace(device, pairs: int, E: int, N: int, K: int) -> int:
-    key = (device.index, pairs, E, N, K)
-    n = _sizes.get(key)
-    if n is None:
-        if len(_sizes) > 4096:  # calls of ever new sizes do not fill the memory
-            _sizes.clear()
-        n = _sizes[key] = experts_workspace_size(pairs, E, N, K)
-    return n

@@ -6,10 +6,12 @@ import contextlib
 
 import torch
 
-from . import _stream
+from . import _check, load
 
 _current = contextlib.nullcontext()
 _scratch: dict = {}
+_sizes: dict = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _COUNTERS = 4096  # arrival counters at the start of a workspace, zero between launches
 
 
@@ -27,7 +29,7 @@ def want(t, name: str, dtype, shape=None, device=None):
 
 
 def want_out(t, name: str, dtype, shape, device):
-    """As `want`, for a tensor that is written in place: contiguous as well."""
+    """As `want`, for a tensor whose memory is used as it lies: contiguous as well."""
     want(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -52,6 +54,24 @@ def on(device, stream, *used):
     return torch.cuda.stream(stream)
 
 
+def run(name: str, device, *args) -> None:
+    """Calls entry point `name` on `device`'s current stream (its last argument)."""
+    status = getattr(load(), name)(*args, _raw_stream(device.index))
+    if status != 0:
+        _check(name, status)
+
+
+def size(query, device, *key) -> int:
+    """A workspace size query, remembered: a pure function of the device and the sizes."""
+    key = (query, device.index, *key)
+    n = _sizes.get(key)
+    if n is None:
+        if len(_sizes) > 4096:  # calls of ever new sizes do not fill the memory
+            _sizes.clear()
+        n = _sizes[key] = query(*key[2:])
+    return n
+
+
 def workspace(need: int, device):
     """A workspace of at least `need` bytes with zeroed arrival counters for a
     launch on the current stream; None for 0.
@@ -66,7 +86,7 @@ def workspace(need: int, device):
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         ws[:_COUNTERS].zero_()
         return ws
-    key = (device.index, _stream(None))
+    key = (device.index, _raw_stream(device.index))
     ws = _scratch.get(key)
     if ws is None or ws.numel() < need:
         ws = torch.empty(need, dtype=torch.uint8, device=device)

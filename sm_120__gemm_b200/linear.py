@@ -9,10 +9,10 @@ from __future__ import annotations
 
 import torch
 
-from . import (ACTIVATIONS, gemm_epilogue_workspace_size, launch_final_epilogue,
-               launch_final_fp32_ws, launch_final_ws, launch_quantize_repack,
-               launch_repack_scales_128, launch_repack_umma, shard_range, workspace_for)
-from .launching import on, want, want_out, workspace
+from . import (ACTIVATIONS, Epilogue, gemm_epilogue_workspace_size, launch_final_fp32_ws,
+               launch_final_ws, launch_quantize_repack, launch_repack_scales_128,
+               launch_repack_umma, shard_range, workspace_for)
+from .launching import on, run, size, want, want_out, workspace
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -121,20 +121,11 @@ class QuantizedLinear:
                 ld = residual.stride(0)
             if out is None:
                 out = torch.empty(M, cols, dtype=dtype, device=dev)
-            ws = workspace(_epilogue_workspace(dev, M, self.N, self.K), dev)
-            launch_final_epilogue(a, self.tiles, self.scales, out, M, self.N, self.K, self.group,
-                                  bias, activation, gated, residual, ld, fp32_out, ws)
+            ws = workspace(size(gemm_epilogue_workspace_size, dev, M, self.N, self.K), dev)
+            e = Epilogue(0 if bias is None else bias.data_ptr(),
+                         0 if residual is None else residual.data_ptr(), ld,
+                         ACTIVATIONS[activation], gated, fp32_out)
+            run("i4g_gemm_epilogue", dev, a.data_ptr(), self.tiles.data_ptr(),
+                self.scales.data_ptr(), out.data_ptr(), M, self.N, self.K, self.group, e,
+                0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
         return out
-
-
-_sizes: dict = {}
-
-
-def _epilogue_workspace(device, M: int, N: int, K: int) -> int:
-    key = (device.index, M, N, K)
-    n = _sizes.get(key)
-    if n is None:
-        if len(_sizes) > 4096:  # calls of ever new sizes do not fill the memory
-            _sizes.clear()
-        n = _sizes[key] = gemm_epilogue_workspace_size(M, N, K)
-    return n
