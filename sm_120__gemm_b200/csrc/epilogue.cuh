@@ -34,6 +34,28 @@ __device__ __forceinline__ float sigmoid_gate(float x, float c0, float c1) {
   return __fdividef(x, 1.0f + __expf(-u));
 }
 
+// GELU x Phi(x) = max(x, 0) - |x| erfc(z) / 2 with z = |x| / sqrt 2: no
+// cancellation on the negative side. erfc(z) exp(z^2) is a polynomial of degree
+// 8 in t = 1 / (1 + z / 2), times t, fitted by weighted least squares for the
+// least largest relative error (4e-8; 3.3e-7 evaluated in FP32): 20
+// instructions, where the library's erfc cost 8 us of a 42 us product (M = 203,
+// N = 14336, whose one wave of tiles hides no epilogue).
+__device__ __forceinline__ float gelu_erf(float x) {
+  const float a = fminf(fabsf(x), 40.0f);  // exp(-800) is 0: infinities keep their limits
+  const float t = __fdividef(1.0f, fmaf(a, 0.35355339f, 1.0f));
+  float p = -0.05889091f;
+  p = fmaf(p, t, 0.28370258f);
+  p = fmaf(p, t, -0.48538491f);
+  p = fmaf(p, t, 0.27597940f);
+  p = fmaf(p, t, -0.02517844f);
+  p = fmaf(p, t, 0.20207012f);
+  p = fmaf(p, t, 0.24326095f);
+  p = fmaf(p, t, 0.28235349f);
+  p = fmaf(p, t, 0.28208768f);
+  const float h = 0.5f * a * (p * t) * __expf(-0.5f * a * a);
+  return x < 0.0f ? -h : x - h;
+}
+
 // Applies the activation to N values; the kind is the same for every thread,
 // so the branch is taken once for all of them.
 template <int N>
@@ -44,7 +66,7 @@ __device__ __forceinline__ void activate(int kind, float (&x)[N]) {
     for (int i = 0; i < N; ++i) x[i] = x[i] < 0.0f ? 0.0f : x[i];  // keeps a NaN
   } else if (kind == kActGelu) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 0.5f * x[i] * erfcf(x[i] * -0.70710678f);
+    for (int i = 0; i < N; ++i) x[i] = gelu_erf(x[i]);
   } else {
     const float c0 = kind == kActSilu ? 1.0f : 1.59576912f;
     const float c1 = kind == kActSilu ? 0.0f : 0.07135482f;

@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 namespace i4g {
 namespace route {
@@ -40,7 +41,14 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kChunk = 128;       // tokens whose choices one bitmap holds
 constexpr int kThreads = 1024;
-constexpr int kOneBlock = 128;    // up to so many tokens one CTA does everything
+constexpr int kOneBlock = 32;     // up to so many tokens one CTA does everything
+// What two FP32 choice scores c <= 1 + |bias| can be off by against each other,
+// relative to max(1, |c|). Sigmoid: p is off by p (1 - p) times exp's error
+// (2 + 1.17 |x| units in the last place, at most 1e-7 so weighted), a
+// reciprocal (1.2e-7) and the bias's addition (6e-8): 5e-7 for two. Softmax: a
+// term's exp (3e-7 weighted by p), and the sum, of at most 16 additions in a
+// lane and 5 across, whose error (21 x 6e-8) scales the difference of the two p.
+constexpr float kSigmoidError = 1e-6f, kSoftmaxError = 2e-6f;
 
 // Order-preserving keys: larger value, larger key; 0 is "not eligible".
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -66,8 +74,12 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
   return (static_cast<uint64_t>(top) << 32) | lo;
 }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+// FP32: the choice's error bound allows for the fast forms; the weights are
+// computed apart (weight_of).
+__device__ __forceinline__ float exp_of(float x) { return __expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float reciprocal(float x) { return __fdividef(1.0f, x); }
+__device__ __forceinline__ double reciprocal(double x) { return 1.0 / x; }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
@@ -83,14 +95,15 @@ template <typename F> struct Key;
 template <> struct Key<float> { using type = uint32_t; };
 template <> struct Key<double> { using type = uint64_t; };
 
-// The scores p of this lane's experts (0 where not eligible).
+// The scores p of this lane's experts (0 where not eligible); returns the
+// softmax's sum of exp(x - top).
 template <typename F, int V>
-__device__ __forceinline__ void scores(const float (&x)[V], float top, int sigmoid, F (&p)[V]) {
+__device__ __forceinline__ F scores(const float (&x)[V], float top, int sigmoid, F (&p)[V]) {
   if (sigmoid) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      p[v] = x[v] > -INFINITY ? F(1) / (F(1) + exp_of(-static_cast<F>(x[v]))) : F(0);
-    return;
+      p[v] = x[v] > -INFINITY ? reciprocal(F(1) + exp_of(-static_cast<F>(x[v]))) : F(0);
+    return F(1);
   }
   F sum = 0;
 #pragma unroll
@@ -105,6 +118,43 @@ __device__ __forceinline__ void scores(const float (&x)[V], float top, int sigmo
   const F r = sum > 0 ? F(1) / sum : F(0);
 #pragma unroll
   for (int v = 0; v < V; ++v) p[v] *= r;
+  return sum;
+}
+
+// The score of a chosen expert, in full FP32 accuracy.
+__device__ __forceinline__ float weight_of(float x, float top, int sigmoid, float sum) {
+  if (sigmoid) return 1.0f / (1.0f + expf(-x));
+  return (x == top ? 1.0f : expf(x - top)) / sum;
+}
+
+// Lane's experts by falling key, the lower index first among equal keys:
+// adjacent exchanges of strictly rising neighbours only, so ties keep their
+// order. `order` holds the registers' first indices, four bits each.
+template <int V>
+using Order = std::conditional_t<(V <= 8), uint32_t, uint64_t>;
+
+template <typename K, int V>
+__device__ __forceinline__ Order<V> sort_keys(K (&key)[V]) {
+  int at[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) at[v] = v;
+#pragma unroll
+  for (int pass = 0; pass < V; ++pass) {
+#pragma unroll
+    for (int v = pass & 1; v + 1 < V; v += 2) {
+      const bool swap = key[v + 1] > key[v];
+      const K k = swap ? key[v + 1] : key[v];
+      key[v + 1] = swap ? key[v] : key[v + 1];
+      key[v] = k;
+      const int a = swap ? at[v + 1] : at[v];
+      at[v + 1] = swap ? at[v] : at[v + 1];
+      at[v] = a;
+    }
+  }
+  Order<V> order = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) order |= static_cast<Order<V>>(at[v]) << (4 * v);
+  return order;
 }
 
 // The choice of one token. On return lane i < top_k holds the i-th expert
@@ -112,139 +162,176 @@ __device__ __forceinline__ void scores(const float (&x)[V], float top, int sigmo
 // max(1, |value|)) decided it; tol = 0 accepts every order.
 template <typename F, int V>
 __device__ __forceinline__ bool choose(const Args& a, int lane, const float (&x)[V],
-                                       const F (&p)[V], bool by_score, F tol, int& my_id) {
+                                       const F (&p)[V], const float (&bias)[V], bool by_score,
+                                       F tol, int& my_id) {
   using K = typename Key<F>::type;
   K key[V];
   const int e0 = lane * V;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const F c = by_score ? p[v] + (a.bias && e0 + v < a.E ? static_cast<F>(a.bias[e0 + v]) : F(0))
-                         : static_cast<F>(x[v]);
+    const F c = by_score ? p[v] + static_cast<F>(bias[v]) : static_cast<F>(x[v]);
     key[v] = x[v] > -INFINITY && c > -INFINITY ? key_of(c) : K(0);
   }
   bool sure = true;
   if (a.n_group > 1) {
     const int size = a.E / a.n_group;
-    // Group scores: lane g holds group g's. A group may start and end inside
-    // a lane, so each group is a pass over the warp.
-    F mine = -INFINITY;
-    for (int g = 0; g < a.n_group; ++g) {
+    const bool whole_lanes = a.E == 32 * V && 32 % a.n_group == 0;
+    const int span = 32 / a.n_group;  // lanes of a group, if it is whole lanes
+    F mine = -INFINITY;               // lane g: group g's score
+    if (whole_lanes) {
+      // the best two of a group's lanes meet in a few exchanges
       K best = 0, second = 0;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int e = e0 + v;
-        const K k = e >= g * size && e < (g + 1) * size ? key[v] : K(0);
-        if (k > best) {
-          second = best;
-          best = k;
-        } else if (k > second) {
-          second = k;
+        second = max(second, min(best, key[v]));
+        best = max(best, key[v]);
+      }
+      for (int d = 1; d < span; d <<= 1) {
+        const K ob = __shfl_xor_sync(kAll, best, d), os = __shfl_xor_sync(kAll, second, d);
+        second = max(max(second, os), min(best, ob));
+        best = max(best, ob);
+      }
+      F score = best ? value_of(best) : -INFINITY;
+      if (a.top2 && second) score += value_of(second);
+      mine = __shfl_sync(kAll, score, (lane * span) & 31);
+    } else {
+      // a group may start and end inside a lane: a pass over the warp for each
+      for (int g = 0; g < a.n_group; ++g) {
+        K best = 0, second = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int e = e0 + v;
+          const K k = e >= g * size && e < (g + 1) * size ? key[v] : K(0);
+          second = max(second, min(best, k));
+          best = max(best, k);
         }
+        const K top = warp_max(best);
+        F score = top ? value_of(top) : -INFINITY;
+        if (a.top2) {
+          const unsigned holders = __ballot_sync(kAll, best == top);
+          const K next = warp_max(lane == __ffs(holders) - 1 ? second : best);
+          if (next) score += value_of(next);
+        }
+        if (lane == g) mine = score;
       }
-      const K top = warp_max(best);
-      F score = top ? value_of(top) : -INFINITY;
-      if (a.top2) {
-        const unsigned holders = __ballot_sync(kAll, best == top);
-        const K next = warp_max(lane == __ffs(holders) - 1 ? second : best);
-        if (next) score += value_of(next);
-      }
-      if (lane == g) mine = score;
     }
     int rank = 0;
-    F lowest_in = INFINITY, highest_out = -INFINITY;
     for (int g = 0; g < a.n_group; ++g) {
       const F other = __shfl_sync(kAll, mine, g);
       rank += other > mine || (other == mine && g < lane);
     }
     const bool kept = lane < a.n_group && rank < a.topk_group;
     const unsigned in = __ballot_sync(kAll, kept);
-    for (int g = 0; g < a.n_group; ++g) {
-      const F s = __shfl_sync(kAll, mine, g);
-      if ((in >> g) & 1) lowest_in = s < lowest_in ? s : lowest_in;
-      else highest_out = s > highest_out ? s : highest_out;
+    if (tol > 0 && by_score && a.topk_group < a.n_group) {
+      // the last group in against the first one out
+      const unsigned at_in = __ballot_sync(kAll, lane < a.n_group && rank == a.topk_group - 1);
+      const unsigned at_out = __ballot_sync(kAll, lane < a.n_group && rank == a.topk_group);
+      const F lowest_in = __shfl_sync(kAll, mine, __ffs(at_in) - 1);
+      const F highest_out = __shfl_sync(kAll, mine, __ffs(at_out) - 1);
+      if (highest_out > -INFINITY)
+        sure = lowest_in - highest_out > 2 * tol * fmax(F(1), fabs(lowest_in));
     }
-    if (tol > 0 && highest_out > -INFINITY && by_score) {
-      const F size_of = fmax(F(1), fabs(lowest_in));
-      sure = lowest_in - highest_out > 2 * tol * size_of;
-    }
+    int g = whole_lanes ? lane / span : e0 / size;
+    int next = whole_lanes ? a.E : (g + 1) * size;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int e = e0 + v;
-      if (e < a.E && !((in >> (e / size)) & 1)) key[v] = 0;
+      if (e0 + v >= next) {
+        ++g;
+        next += size;
+      }
+      if (!((in >> (g & 31)) & 1)) key[v] = 0;
     }
   }
+  Order<V> order = sort_keys(key);
   my_id = -1;
-  K last = 0;
+  K my_key = 0, past = 0;  // lane i: the i-th key chosen; the first one not chosen
   const int rounds = a.top_k + (tol > 0 && by_score ? 1 : 0);
   for (int i = 0; i < rounds; ++i) {
-    K best = 0;
-    int at = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > best) {
-        best = key[v];
-        at = v;
-      }
-    const K top = warp_max(best);
+    const K top = warp_max(key[0]);
     if (top == 0) break;  // none left
-    if (tol > 0 && by_score && i > 0) {
-      const F hi = value_of(last), lo = value_of(top);
-      if (!(hi - lo > tol * fmax(F(1), fabs(hi)))) sure = false;
+    if (i == a.top_k) {
+      past = top;
+      break;
     }
-    last = top;
-    const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
-    const int id = __shfl_sync(kAll, e0 + at, winner);
-    if (lane == i && i < a.top_k) my_id = id;
+    const int winner = __ffs(__ballot_sync(kAll, key[0] == top)) - 1;
+    const int id = __shfl_sync(kAll, e0 + static_cast<int>(order & 15), winner);
+    if (lane == i) {
+      my_id = id;
+      my_key = top;
+    }
+    if (lane == winner) {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (lane == winner && v == at) key[v] = 0;
+      for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
+      key[V - 1] = 0;
+      order >>= 4;
+    }
+  }
+  if (tol > 0 && by_score) {
+    K next = __shfl_down_sync(kAll, my_key, 1);
+    if (lane == a.top_k - 1 || lane == 31) next = past;
+    bool close = false;
+    if (my_key && next) {
+      const F hi = value_of(my_key), lo = value_of(next);
+      close = !(hi - lo > tol * fmax(F(1), fabs(hi)));
+    }
+    sure = sure && !__any_sync(kAll, close);
   }
   return sure;
 }
 
-// Token t's experts and weights, by one warp; lane i < top_k returns expert i.
-template <int V, bool FP32>
-__device__ __forceinline__ int route_token(const Args& a, int t, int lane) {
-  float x[V];
+// This lane's entries of a row of E (logits or bias); `none` past the last.
+template <int V, typename T>
+__device__ __forceinline__ void load_lane(const T* row, int E, int lane, float none,
+                                          float (&x)[V]) {
   const int e0 = lane * V;
+  if constexpr (V % 4 == 0 && sizeof(T) == 4) {
+    if (E == 32 * V && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    x[v] = -INFINITY;
-    if (e0 + v < a.E) {
-      const size_t at = static_cast<size_t>(t) * a.ld + e0 + v;
-      x[v] = FP32 ? static_cast<const float*>(a.logits)[at]
-                  : __half2float(static_cast<const __half*>(a.logits)[at]);
+      for (int q = 0; q < V / 4; ++q) {
+        const float4 f = reinterpret_cast<const float4*>(row + e0)[q];
+        x[4 * q] = f.x;
+        x[4 * q + 1] = f.y;
+        x[4 * q + 2] = f.z;
+        x[4 * q + 3] = f.w;
+      }
+      return;
     }
   }
+#pragma unroll
+  for (int v = 0; v < V; ++v) x[v] = e0 + v < E ? static_cast<float>(row[e0 + v]) : none;
+}
+
+template <bool FP32>
+__device__ __forceinline__ auto logits_of(const Args& a, int t) {
+  using T = std::conditional_t<FP32, float, __half>;
+  return static_cast<const T*>(a.logits) + static_cast<size_t>(t) * a.ld;
+}
+
+// Token t's experts and weights from this lane's logits x, by one warp; lane i < top_k returns expert i.
+template <int V, bool FP32>
+__device__ __forceinline__ int route_token(const Args& a, int t, int lane,
+                                           const float (&bias)[V], const float (&x)[V]) {
   float top = -INFINITY;
 #pragma unroll
   for (int v = 0; v < V; ++v) top = x[v] > top ? x[v] : top;
 #pragma unroll
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
   float p[V];
-  scores(x, top, a.sigmoid, p);
+  const float sum = scores(x, top, a.sigmoid, p);
   const bool by_score = a.bias || (a.n_group > 1 && a.top2);
   int id;
-  if (!choose(a, lane, x, p, by_score, 2e-6f, id)) {
+  if (!choose(a, lane, x, p, bias, by_score, a.sigmoid ? kSigmoidError : kSoftmaxError,
+              id)) {
     double pd[V];
     scores(x, top, a.sigmoid, pd);
-    choose(a, lane, x, pd, by_score, 0.0, id);
+    choose(a, lane, x, pd, bias, by_score, 0.0, id);
   }
-  // lane i's weight is expert id's p
-  float w = 0.0f;
-  for (int i = 0; i < a.top_k; ++i) {
-    const int want = __shfl_sync(kAll, id, i);
-    if (want < 0) break;
-    float mine = 0.0f;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (e0 + v == want) mine = p[v];
-    mine = __shfl_sync(kAll, mine, want / V);
-    if (lane == i) w = mine;
-  }
+  float w = 0.0f;  // lane i: expert id's score
+  if (id >= 0)
+    w = weight_of(static_cast<float>(logits_of<FP32>(a, t)[id]), top, a.sigmoid, sum);
   if (a.renormalize) {
-    const float sum = warp_sum(lane < a.top_k ? w : 0.0f);
-    w = sum > 0.0f ? w / sum : 0.0f;
+    const float all = warp_sum(w);
+    w = all > 0.0f ? w / all : 0.0f;
   }
   if (lane < a.top_k) {
     const size_t at = static_cast<size_t>(t) * a.top_k + lane;
@@ -262,7 +349,7 @@ __device__ __forceinline__ int first_token(int T, int b, int nb) {
 // A CTA's shared tables while it places pairs.
 struct Place {
   int base[kMaxExperts];                      // next row of each expert
-  uint32_t bits[kMaxExperts][kChunk / 32];    // tokens of the chunk that chose it
+  alignas(16) uint32_t bits[kMaxExperts][kChunk / 32];  // tokens of the chunk that chose it
   int warp_total[32];
 };
 
@@ -277,12 +364,9 @@ __device__ __forceinline__ int block_scan(int v, int* warp_total, int& total) {
   }
   if (lane == 31) warp_total[warp] = sum;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) {
-    if (i < warp) before += warp_total[i];
-    total += warp_total[i];
-  }
+  int mine = lane < static_cast<int>(blockDim.x) / 32 ? warp_total[lane] : 0;
+  total = __reduce_add_sync(kAll, mine);
+  const int before = __reduce_add_sync(kAll, lane < warp ? mine : 0);
   return before + sum - v;
 }
 
@@ -292,34 +376,47 @@ __device__ __forceinline__ int block_scan(int v, int* warp_total, int& total) {
 // (a token chooses an expert once), so the order is by token and nothing
 // depends on which thread comes first.
 __device__ __forceinline__ void place_pairs(const Args& a, Place& s, int t0, int t1) {
+  constexpr int kMost = kChunk * kMaxTopK / kThreads;  // pairs of a chunk per thread
   for (int c0 = t0; c0 < t1; c0 += kChunk) {
-    const int n = min(kChunk, t1 - c0);
-    for (int i = threadIdx.x; i < a.E * (kChunk / 32); i += blockDim.x)
-      (&s.bits[0][0])[i] = 0u;
-    __syncthreads();
-    const int pairs = n * a.top_k;
+    const int pairs = min(kChunk, t1 - c0) * a.top_k;
     const size_t p0 = static_cast<size_t>(c0) * a.top_k;
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-      const int e = a.ids[p0 + i], t = i / a.top_k;
-      if (e >= 0) atomicOr(&s.bits[e][t >> 5], 1u << (t & 31));
+    int e[kMost], t[kMost];
+#pragma unroll
+    for (int q = 0; q < kMost; ++q) {
+      const int i = threadIdx.x + q * kThreads;
+      e[q] = i < pairs ? a.ids[p0 + i] : -1;
+      t[q] = i / a.top_k;
     }
+    for (int i = threadIdx.x; i < a.E * (kChunk / 32); i += kThreads) (&s.bits[0][0])[i] = 0u;
     __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-      const int e = a.ids[p0 + i], t = i / a.top_k;
+#pragma unroll
+    for (int q = 0; q < kMost; ++q)
+      if (e[q] >= 0) atomicOr(&s.bits[e[q]][t[q] >> 5], 1u << (t[q] & 31));
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kMost; ++q) {
+      const int i = threadIdx.x + q * kThreads;
+      if (i >= pairs) break;
       int row = -1;
-      if (e >= 0) {
-        row = s.base[e] + __popc(s.bits[e][t >> 5] & ((1u << (t & 31)) - 1u));
-        for (int q = 0; q < (t >> 5); ++q) row += __popc(s.bits[e][q]);
+      if (e[q] >= 0) {
+        const uint4 b = *reinterpret_cast<const uint4*>(s.bits[e[q]]);
+        const uint32_t word[4] = {b.x, b.y, b.z, b.w};
+        const uint32_t below = (1u << (t[q] & 31)) - 1u;
+        row = s.base[e[q]];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          row += __popc(word[w] & (w < (t[q] >> 5) ? ~0u : (w == (t[q] >> 5) ? below : 0u)));
         a.rows[row] = static_cast<int>(p0) + i;
       }
       a.slots[p0 + i] = row;
     }
+    if (c0 + kChunk >= t1) break;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    for (int x = threadIdx.x; x < a.E; x += kThreads) {
       int count = 0;
 #pragma unroll
-      for (int q = 0; q < kChunk / 32; ++q) count += __popc(s.bits[e][q]);
-      s.base[e] += count;
+      for (int q = 0; q < kChunk / 32; ++q) count += __popc(s.bits[x][q]);
+      s.base[x] += count;
     }
     __syncthreads();
   }
@@ -334,8 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1) route_small_kernel(const Args a) 
   grid_dependency_wait();
   if (threadIdx.x == 0) launch_dependents();
   __syncthreads();
+  float bias[V] = {};
+  if (a.bias) load_lane(a.bias, a.E, lane, 0.0f, bias);
   for (int t = warp; t < a.T; t += blockDim.x / 32) {
-    const int e = route_token<V, FP32>(a, t, lane);
+    float x[V];
+    load_lane(logits_of<FP32>(a, t), a.E, lane, -INFINITY, x);
+    const int e = route_token<V, FP32>(a, t, lane, bias, x);
     if (lane < a.top_k && e >= 0) atomicAdd(&s.base[e], 1);
   }
   __syncthreads();
@@ -348,13 +449,14 @@ __global__ void __launch_bounds__(kThreads, 1) route_small_kernel(const Args a) 
     a.offsets[e] = before;
   }
   if (e == 0) a.offsets[a.E] = total;
-  __syncthreads();
+  __syncthreads();  // also orders the ids just written before they are read
   place_pairs(a, s, 0, a.T);
   for (int i = total + threadIdx.x; i < a.T * a.top_k; i += blockDim.x) a.rows[i] = -1;
 }
 
 // First of two kernels: choices, and how many of the block's pairs each
-// expert got (counts [block][E], 16 bits each: a block has fewer tokens).
+// expert got (counts [block][E rounded up to even], 16 bits each: a block has
+// fewer tokens than that).
 template <int V, bool FP32>
 __global__ void __launch_bounds__(kThreads, 1)
     route_choose_kernel(const Args a, uint16_t* __restrict__ counts) {
@@ -366,13 +468,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   const int t0 = first_token(a.T, blockIdx.x, gridDim.x);
   const int t1 = first_token(a.T, blockIdx.x + 1, gridDim.x);
-  for (int t = t0 + warp; t < t1; t += blockDim.x / 32) {
-    const int e = route_token<V, FP32>(a, t, lane);
+  float bias[V] = {};
+  if (a.bias) load_lane(a.bias, a.E, lane, 0.0f, bias);
+  float next[V];
+  if (t0 + warp < t1) load_lane(logits_of<FP32>(a, t0 + warp), a.E, lane, -INFINITY, next);
+  for (int t = t0 + warp; t < t1; t += kThreads / 32) {
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = next[v];
+    // the next token's logits arrive while this one's are sorted
+    if (t + kThreads / 32 < t1)
+      load_lane(logits_of<FP32>(a, t + kThreads / 32), a.E, lane, -INFINITY, next);
+    const int e = route_token<V, FP32>(a, t, lane, bias, x);
     if (lane < a.top_k && e >= 0) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x)
-    counts[static_cast<size_t>(blockIdx.x) * a.E + e] = static_cast<uint16_t>(count[e]);
+  const int width = (a.E + 1) & ~1;
+  for (int e = threadIdx.x; e < width; e += blockDim.x)
+    counts[static_cast<size_t>(blockIdx.x) * width + e] = static_cast<uint16_t>(count[e]);
 }
 
 // Second kernel: every block adds the counts up itself (all of them for the
@@ -387,18 +500,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) launch_dependents();
   __syncthreads();
   const int nb = gridDim.x, b = blockIdx.x;
-  const int lanes = max(1, static_cast<int>(blockDim.x) / a.E);  // threads per expert
-  const int e = threadIdx.x % a.E, part = threadIdx.x / a.E;
-  if (part < lanes) {
-    int before = 0, sum = 0;
-#pragma unroll 8
-    for (int i = part; i < nb; i += lanes) {
-      const int c = counts[static_cast<size_t>(i) * a.E + e];
-      sum += c;
-      before += i < b ? c : 0;
+  // two experts a thread, all its loads in flight together
+  const int pairs_of = (a.E + 1) / 2;
+  const int parts = static_cast<int>(blockDim.x) / pairs_of;
+  const int e2 = threadIdx.x % pairs_of, part = threadIdx.x / pairs_of;
+  if (part < parts) {
+    const uint32_t* col = reinterpret_cast<const uint32_t*>(counts) + e2;
+    int before0 = 0, before1 = 0, sum0 = 0, sum1 = 0;
+#pragma unroll 20
+    for (int i = part; i < nb; i += parts) {
+      const uint32_t c = col[static_cast<size_t>(i) * pairs_of];
+      const int c0 = static_cast<int>(c & 0xffffu), c1 = static_cast<int>(c >> 16);
+      sum0 += c0;
+      sum1 += c1;
+      before0 += i < b ? c0 : 0;
+      before1 += i < b ? c1 : 0;
     }
-    atomicAdd(&all[e], sum);  // integers: the order does not matter
-    atomicAdd(&s.base[e], before);
+    // integers: the order of the additions does not matter
+    atomicAdd(&all[2 * e2], sum0);
+    atomicAdd(&s.base[2 * e2], before0);
+    if (2 * e2 + 1 < a.E) {
+      atomicAdd(&all[2 * e2 + 1], sum1);
+      atomicAdd(&s.base[2 * e2 + 1], before1);
+    }
   }
   __syncthreads();
   int total;
@@ -512,7 +636,7 @@ __global__ void __launch_bounds__(kCombineThreads)
 
 size_t workspace_bytes(int T, int E, int sm_count) {
   if (T <= kOneBlock) return 0;
-  return static_cast<size_t>(blocks_for(T, sm_count)) * E * sizeof(uint16_t);
+  return static_cast<size_t>(blocks_for(T, sm_count)) * ((E + 1) & ~1) * sizeof(uint16_t);
 }
 
 cudaError_t launch(const Args& a, bool fp32_logits, int sm_count, void* workspace,
