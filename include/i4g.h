@@ -146,8 +146,7 @@ int i4g_gemm_variant(const void* A, const uint8_t* tiles, const void* scales,
  * points share the tiles of the last, partial wave out along K over all SMs
  * (each leftover tile split 2 to 4 ways; with the I4G_STREAMK=1 environment
  * variable, read at the first launch, stream-K where it is cheaper: equal
- * shares of the leftover tiles' 64-k blocks, one per CTA; opt-in because it
- * gave an intermittently wrong tile on B200, a race not yet found) and
+ * shares of the leftover tiles' 64-k blocks, one per CTA) and
  * reduce the FP32 partial tiles through a caller-owned workspace, in a fixed
  * order, so results are bitwise reproducible and within the usual FP32
  * accumulation tolerance of the unsplit kernel. The decode kernel (M <= 16,

@@ -675,8 +675,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb1) : "r"(ssrc + TILE_N * 2));
       else
         sb1 = sb0;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(wempty(s));
       const uint32_t s0 = half_bits_x2(sb0), s1 = half_bits_x2(sb1);
       uint32_t r[32];
       const uint32_t wv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
@@ -710,7 +708,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tfull(ts));
+        if (lane == 0) {
+          mbar_arrive(tfull(ts));
+          mbar_arrive(wempty(s));
+        }
       } else {
         if (!free) break;
         tc_fence_after();
@@ -718,6 +719,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(tfull(ts));
+        // The packed slot is given back only once the stores above have used
+        // what was loaded from it: an arrival right after the loads can
+        // overtake them (they queue behind the epilogue's global stores, the
+        // arrival does not) and let the next copy into the slot land under
+        // them. With partial tiles stored while the pipeline runs (the
+        // stream-K tail) that gave an intermittently wrong tile.
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wempty(s));
       }
     }
   } else {
@@ -955,10 +964,10 @@ int pair_mode() {
   return v;
 }
 
-// The stream-K tail is opt-in (I4G_STREAMK=1, read once): on B200 it gave an
-// intermittently wrong output tile (about one launch in 12-16 at
-// M = 1024, N = 3200, K = 12288, where every CTA owns two partial tiles), a
-// race not yet found; whole tiles and equal splits were exact in every run.
+// The stream-K tail is opt-in (I4G_STREAMK=1, read once): equal splits were
+// measured without it. (It once gave an intermittently wrong output tile: a
+// packed-weight slot was given back before its last read, see the dequant
+// warps; exact in 200 of 200 launches at M = 1024, N = 3200, K = 12288 since.)
 int streamk_mode() {
   static const int v = [] {
     const char* e = std::getenv("I4G_STREAMK");
