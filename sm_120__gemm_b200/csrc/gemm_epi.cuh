@@ -196,8 +196,9 @@ __device__ __forceinline__ bool item_at(const Walk& w, int j, Item& r) {
   }
   const int first = w.offsets ? w.table[e] : 0;
   const int num_m = w.offsets ? w.table[e + 1] - first : w.num_m;
-  int mt;
-  tile_coords(tile - first * w.num_n, num_m, w.num_n, mt, r.nt);
+  int mt = 0;
+  r.nt = tile - first * w.num_n;
+  if (num_m > 1) tile_coords(r.nt, num_m, w.num_n, mt, r.nt);
   r.e = e;
   int begin = 0, end = w.M;
   if (w.offsets) {
@@ -426,15 +427,17 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
       for (int u = u0; u < u1; ++u) {
         ok = mbar_wait_warp(empty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
         if (!ok) break;
-        const int nb = min(L::BS, kblocks - u * L::BS);
         const uint32_t dst = act_base + s * L::ACT_BYTES;
-        if (elect_one()) {
-          // a box past the last block (the unit's second, of an odd K / 64)
-          // reads zeros and counts its bytes like any other
-          mbar_arrive_expect_tx(full(s), a.rows ? nb * quads * 512 : L::ACT_BYTES);
-          if (!a.rows) tma_load_3d(dst, &act_map, full(s), 0, row0, u * L::BS);
-        }
-        if (a.rows) {
+        if (!a.rows) {
+          // a box past the last block (in the last unit, if K / 64 is not a
+          // multiple of BS) reads zeros and counts its bytes like any other
+          if (elect_one()) {
+            mbar_arrive_expect_tx(full(s), L::ACT_BYTES);
+            tma_load_3d(dst, &act_map, full(s), 0, row0, u * L::BS);
+          }
+        } else {
+          const int nb = min(L::BS, kblocks - u * L::BS);
+          if (elect_one()) mbar_arrive_expect_tx(full(s), nb * quads * 512);
           __syncwarp();
           for (int b = 0; b < nb; ++b)
 #pragma unroll
@@ -461,22 +464,30 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     Item w;
     for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
       const size_t col = uniform(static_cast<uint32_t>(w.e * num_n + w.nt));  // 128-column run
-      const uint8_t* wsrc = a.tiles + col * kblocks * WBLOCK_BYTES;
-      const __half* ssrc = a.scales + col * groups * TILE_N;
       const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
+      const int kb0 = u0 * L::BS;
+      const uint8_t* wsrc = a.tiles + (col * kblocks + kb0) * WBLOCK_BYTES;
+      const __half* ssrc = a.scales + (col * groups + kb0 * BK / GROUP) * TILE_N;
       for (int u = u0; u < u1; ++u) {
         ok = mbar_wait_warp(wempty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
         if (!ok) break;
-        if (elect_one()) {
-          const int kb = u * L::BS, nb = min(L::BS, kblocks - kb);
-          const int g0 = kb * BK / GROUP, g1 = ((kb + nb) * BK + GROUP - 1) / GROUP;
-          const uint32_t dst = w_base + s * L::W_SLOT;
-          mbar_arrive_expect_tx(wfull(s), nb * WBLOCK_BYTES + (g1 - g0) * 256);
-          bulk_load(dst, wsrc + static_cast<size_t>(kb) * WBLOCK_BYTES, nb * WBLOCK_BYTES,
-                    wfull(s));
-          bulk_load(dst + L::BS * WBLOCK_BYTES, ssrc + static_cast<size_t>(g0) * TILE_N,
-                    (g1 - g0) * 256, wfull(s));
+        // a whole unit's sizes are constants; one that starts inside a group
+        // of 128 (one block a unit) still needs that group
+        constexpr uint32_t kGroupsFull = (L::BS * BK + GROUP - 1) / GROUP;
+        uint32_t wbytes = L::BS * WBLOCK_BYTES, sbytes = kGroupsFull * TILE_N * 2;
+        if (L::BS > 1 && u == kunits - 1) {
+          const uint32_t nb = kblocks - u * L::BS;
+          wbytes = nb * WBLOCK_BYTES;
+          sbytes = (nb * BK + GROUP - 1) / GROUP * TILE_N * 2;
         }
+        if (elect_one()) {
+          const uint32_t dst = w_base + s * L::W_SLOT;
+          mbar_arrive_expect_tx(wfull(s), wbytes + sbytes);
+          bulk_load(dst, wsrc, wbytes, wfull(s));
+          bulk_load(dst + L::BS * WBLOCK_BYTES, ssrc, sbytes, wfull(s));
+        }
+        wsrc += L::BS * WBLOCK_BYTES;
+        if (L::BS * BK >= GROUP || (u & 1)) ssrc += kGroupsFull * TILE_N;
         ++issued;
         if (++s == static_cast<uint32_t>(W_STAGES)) {
           s = 0;
@@ -490,19 +501,25 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issue
-    // Every loop bound is warp-uniform (see elect_one, uniform). A tile's MMAs
-    // are as wide as its rows (rounded up to 16); wider ones would only take
-    // longer.
+    // Every loop bound is warp-uniform (see elect_one, uniform). The MMAs of a
+    // tall tile are as wide as its rows (rounded up to 16); below 64 rows the
+    // width costs no time and finding the rows would.
     const uint64_t b_desc0 = smem_desc_sw128(act_base);
     uint32_t s = 0, ph = 0;
     uint32_t used[2] = {0, 0};  // segments committed per accumulator
     int acc = 0;
     bool ok = true;
     Item w;
-    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
+    for (int j = 0; ok; ++j) {
+      uint32_t idesc = idesc_f16_f32(TILE_N, TILE_M);
+      if constexpr (TILE_M > 64) {
+        if (!__any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w))) break;
+        idesc = idesc_f16_f32(TILE_N, static_cast<int>(uniform((w.rows + 15) & ~15)));
+      } else {
+        if (!__any_sync(0xffffffffu, span_at(walk, j, w.u0, w.u1))) break;
+      }
       const int u1 = static_cast<int>(uniform(w.u1));
       int u = static_cast<int>(uniform(w.u0));
-      const uint32_t idesc = idesc_f16_f32(TILE_N, static_cast<int>(uniform((w.rows + 15) & ~15)));
       const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
       uint32_t accumulate = 0;  // the item's first MMA starts the sum
       while (true) {
@@ -519,14 +536,23 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
           tc_fence_after();
           const uint64_t b_desc = b_desc0 + ((s * L::ACT_BYTES) >> 4);
           const uint32_t a_tmem = tmem_base + s * L::T_STAGE;
-#pragma unroll
-          for (int b = 0; b < L::BS; ++b) {
-            if (b > 0 && u * L::BS + b >= kblocks) break;
-            mma_f16_ts_block(d_tmem, a_tmem + b * T_COLS, b_desc + ((b * L::BOX_BYTES) >> 4),
-                             idesc, accumulate);
-            accumulate = 1;
+          if (u * L::BS + L::BS <= kblocks) {
+            if constexpr (L::BS == 4)
+              mma_f16_ts_blocks4(d_tmem, a_tmem, b_desc, idesc, accumulate, L::BOX_BYTES >> 4,
+                                 empty(s));
+            else if constexpr (L::BS == 2)
+              mma_f16_ts_blocks2(d_tmem, a_tmem, b_desc, idesc, accumulate, L::BOX_BYTES >> 4,
+                                 empty(s));
+            else
+              mma_f16_ts_blocks1(d_tmem, a_tmem, b_desc, idesc, accumulate, empty(s));
+          } else {
+            // the last unit's blocks
+            for (int b = 0; u * L::BS + b < kblocks; ++b)
+              mma_f16_ts_block(d_tmem, a_tmem + b * T_COLS, b_desc + ((b * L::BOX_BYTES) >> 4),
+                               idesc, b == 0 ? accumulate : 1u);
+            if (elect_one()) tc_commit(empty(s));
           }
-          if (elect_one()) tc_commit(empty(s));
+          accumulate = 1;
           if (++s == static_cast<uint32_t>(STAGES)) {
             s = 0;
             ph ^= 1u;
@@ -547,90 +573,90 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     const int row = quarter * 32 + lane;  // weight column inside the tile
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const NibbleMask nibble;
-    int ws = 0, ts = 0;
-    uint32_t wph = 0, tph = 0, turn = 0;
+    // this group's units: dgroup, dgroup + DEQ, ... of the CTA's
+    const int total = static_cast<int>(uniform(walk.units()));
+    const int whole_units = walk.whole * kunits;
+    uint32_t ws = dgroup % W_STAGES, wph = (dgroup / W_STAGES) & 1u;
+    uint32_t ts = dgroup % STAGES, tph = (dgroup / STAGES) & 1u;
     bool ok = true;
-    Item w;
-    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
-      const int u1 = static_cast<int>(uniform(w.u1));
-      for (int u = static_cast<int>(uniform(w.u0)); u < u1; ++u) {
-        if (turn == dgroup) {
-          ok = mbar_wait_warp(wfull(ws), wph, abort_flag, a.status, a.wait_limit_ns);
-          if (!ok) break;
-          const uint32_t slot = w_base + ws * L::W_SLOT;
+    for (int it = static_cast<int>(dgroup); it < total; it += L::DEQ) {
+      int nb = L::BS;
+      if (L::BS > 1 && kblocks % L::BS != 0) {
+        const int at = it < whole_units ? it : it - whole_units + walk.c0;
+        nb = min(nb, kblocks - static_cast<int>(uniform(at % kunits)) * L::BS);
+      }
+      ok = mbar_wait_warp(wfull(ws), wph, abort_flag, a.status, a.wait_limit_ns);
+      if (!ok) break;
+      const uint32_t slot = w_base + ws * L::W_SLOT;
 #pragma unroll
-          for (int b = 0; b < L::BS; ++b) {
-            if (L::BS > 1 && b > 0 && u * L::BS + b >= kblocks) break;
-            const uint32_t wsrc = slot + b * WBLOCK_BYTES + row * 16;
-            uint4 c0, c1;
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(c0.x), "=r"(c0.y), "=r"(c0.z), "=r"(c0.w)
-                         : "r"(wsrc));
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(c1.x), "=r"(c1.y), "=r"(c1.z), "=r"(c1.w)
-                         : "r"(wsrc + 2048));
-            uint16_t sb0, sb1;
-            // the block's first scale group inside the unit (a group of 128
-            // holds both blocks of a unit)
-            constexpr int kGroups = GROUP == 32 ? 2 : 1;
-            const uint32_t ssrc = slot + L::BS * WBLOCK_BYTES +
-                                  (GROUP == 128 ? b / 2 : b * kGroups) * (TILE_N * 2) + row * 2;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb0) : "r"(ssrc));
-            if (GROUP == 32)
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb1) : "r"(ssrc + TILE_N * 2));
-            else
-              sb1 = sb0;
-            const uint32_t s0 = half_bits_x2(sb0), s1 = half_bits_x2(sb1);
-            uint32_t r[32];
-            const uint32_t wv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-            if (__all_sync(0xffffffffu,
-                           fast_scale(sb0) && (GROUP != 32 || fast_scale(sb1)))) {
+      for (int b = 0; b < L::BS; ++b) {
+        if (b > 0 && b >= nb) break;
+        const uint32_t wsrc = slot + b * WBLOCK_BYTES + row * 16;
+        uint4 c0, c1;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(c0.x), "=r"(c0.y), "=r"(c0.z), "=r"(c0.w)
+                     : "r"(wsrc));
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(c1.x), "=r"(c1.y), "=r"(c1.z), "=r"(c1.w)
+                     : "r"(wsrc + 2048));
+        uint16_t sb0, sb1;
+        // the block's first scale group inside the unit
+        const uint32_t ssrc = slot + L::BS * WBLOCK_BYTES +
+                              (b * BK / GROUP) * (TILE_N * 2) + row * 2;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb0) : "r"(ssrc));
+        if (GROUP == 32)
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sb1) : "r"(ssrc + TILE_N * 2));
+        else
+          sb1 = sb0;
+        const uint32_t s0 = half_bits_x2(sb0), s1 = half_bits_x2(sb1);
+        uint32_t r[32];
+        const uint32_t wv[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        if (__all_sync(0xffffffffu, fast_scale(sb0) && (GROUP != 32 || fast_scale(sb1)))) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                decode_word(wv[i], (i < 4 ? s0 : s1) + kTimes2p20,
-                            (i < 4 ? s0 : s1) + kTimesMinus8, nibble, &r[4 * i]);
-            } else {
+          for (int i = 0; i < 8; ++i)
+            decode_word(wv[i], (i < 4 ? s0 : s1) + kTimes2p20, (i < 4 ? s0 : s1) + kTimesMinus8,
+                        nibble, &r[4 * i]);
+        } else {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t sc = i < 4 ? s0 : s1;
-                r[4 * i + 0] = decode_pair<0>(wv[i], sc);
-                r[4 * i + 1] = decode_pair<1>(wv[i], sc);
-                r[4 * i + 2] = decode_pair<2>(wv[i], sc);
-                r[4 * i + 3] = decode_pair<3>(wv[i], sc);
-              }
-            }
-            if (b == 0) {
-              ok = mbar_wait_warp(empty(ts), tph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            tmem_st_32x32b_x32(tmem_base + lane_addr + ts * L::T_STAGE + b * T_COLS, r);
-          }
-          if (!ok) break;
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(full(ts));
-            // The packed slot is given back only now: the TMEM store has
-            // consumed what was loaded from it. An arrival right after the
-            // loads can overtake them (they queue behind the epilogue's global
-            // stores, the arrival does not), and the next copy into the slot
-            // then overtakes the loads: one 64-k block of some columns was
-            // wrong in every second launch of M = 1024, N = 2048, K = 12288,
-            // where partial tiles are stored while the pipeline runs.
-            mbar_arrive(wempty(ws));
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t sc = i < 4 ? s0 : s1;
+            r[4 * i + 0] = decode_pair<0>(wv[i], sc);
+            r[4 * i + 1] = decode_pair<1>(wv[i], sc);
+            r[4 * i + 2] = decode_pair<2>(wv[i], sc);
+            r[4 * i + 3] = decode_pair<3>(wv[i], sc);
           }
         }
-        if (++turn == L::DEQ) turn = 0;
-        if (++ws == W_STAGES) {
-          ws = 0;
-          wph ^= 1u;
+        if (b == 0) {
+          ok = mbar_wait_warp(empty(ts), tph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
+          if (!ok) break;
+          tc_fence_after();
         }
-        if (++ts == STAGES) {
-          ts = 0;
-          tph ^= 1u;
-        }
+        tmem_st_32x32b_x32(tmem_base + lane_addr + ts * L::T_STAGE + b * T_COLS, r);
+      }
+      if (!ok) break;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full(ts));
+        // The packed slot is given back only now: the TMEM store has consumed
+        // what was loaded from it. An arrival right after the loads can
+        // overtake them (they queue behind the epilogue's global stores, the
+        // arrival does not), and the next copy into the slot then overtakes
+        // the loads: one 64-k block of some columns was wrong in every second
+        // launch of M = 1024, N = 2048, K = 12288, where partial tiles are
+        // stored while the pipeline runs.
+        mbar_arrive(wempty(ws));
+      }
+      ws += L::DEQ;
+      if (ws >= static_cast<uint32_t>(W_STAGES)) {
+        ws -= W_STAGES;
+        wph ^= 1u;
+      }
+      ts += L::DEQ;
+      while (ts >= static_cast<uint32_t>(STAGES)) {
+        ts -= STAGES;
+        tph ^= 1u;
       }
     }
   } else {

@@ -511,6 +511,66 @@ __device__ __forceinline__ void mma_f16_ts_block(uint32_t d_tmem, uint32_t a_tme
       : "memory");
 }
 
+// All MMAs of a ring stage of whole 64-k blocks (operand A 32 TMEM columns per
+// block, operand B `box` 16-byte units apart) and the commit that frees it, by
+// one elected lane of a converged warp.
+#define I4G_MMA_STEP(A, B, ACC) \
+  "add.u32 a, %1, " A ";\n\t" \
+  "add.u64 b, t, " B ";\n\t" \
+  "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, " ACC ";\n\t"
+#define I4G_MMA_BLOCK(A0, A1, A2, A3, ACC)                                 \
+  I4G_MMA_STEP(A0, "0", ACC) I4G_MMA_STEP(A1, "2", "yes")                  \
+  I4G_MMA_STEP(A2, "4", "yes") I4G_MMA_STEP(A3, "6", "yes")
+#define I4G_MMA_HEAD                             \
+  "{\n\t.reg .pred one, acc, yes;\n\t"          \
+  ".reg .b32 a;\n\t"                             \
+  ".reg .b64 b, t;\n\t"                          \
+  "elect.sync _|one, 0xffffffff;\n\t"            \
+  "setp.ne.b32 acc, %4, 0;\n\t"                  \
+  "setp.eq.b32 yes, 0, 0;\n\t"                   \
+  "mov.b64 t, %2;\n\t"
+#define I4G_MMA_NEXT "add.u64 t, t, %6;\n\t"
+#define I4G_MMA_COMMIT                                                                   \
+  "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+
+__device__ __forceinline__ void mma_f16_ts_blocks1(uint32_t d_tmem, uint32_t a_tmem,
+                                                   uint64_t b_desc, uint32_t idesc,
+                                                   uint32_t accumulate, uint32_t bar) {
+  asm volatile(I4G_MMA_HEAD I4G_MMA_BLOCK("0", "8", "16", "24", "acc") I4G_MMA_COMMIT ::"r"(
+                   d_tmem),
+               "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ void mma_f16_ts_blocks2(uint32_t d_tmem, uint32_t a_tmem,
+                                                   uint64_t b_desc, uint32_t idesc,
+                                                   uint32_t accumulate, uint64_t box,
+                                                   uint32_t bar) {
+  asm volatile(I4G_MMA_HEAD I4G_MMA_BLOCK("0", "8", "16", "24", "acc") I4G_MMA_NEXT
+                   I4G_MMA_BLOCK("32", "40", "48", "56", "yes") I4G_MMA_COMMIT ::"r"(d_tmem),
+               "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(bar), "l"(box)
+               : "memory");
+}
+
+__device__ __forceinline__ void mma_f16_ts_blocks4(uint32_t d_tmem, uint32_t a_tmem,
+                                                   uint64_t b_desc, uint32_t idesc,
+                                                   uint32_t accumulate, uint64_t box,
+                                                   uint32_t bar) {
+  asm volatile(I4G_MMA_HEAD I4G_MMA_BLOCK("0", "8", "16", "24", "acc") I4G_MMA_NEXT
+                   I4G_MMA_BLOCK("32", "40", "48", "56", "yes") I4G_MMA_NEXT
+                       I4G_MMA_BLOCK("64", "72", "80", "88", "yes") I4G_MMA_NEXT
+                           I4G_MMA_BLOCK("96", "104", "112", "120", "yes") I4G_MMA_COMMIT ::"r"(
+                               d_tmem),
+               "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(bar), "l"(box)
+               : "memory");
+}
+
+#undef I4G_MMA_STEP
+#undef I4G_MMA_BLOCK
+#undef I4G_MMA_HEAD
+#undef I4G_MMA_NEXT
+#undef I4G_MMA_COMMIT
+
 // Shared-memory matrix descriptor for a K-major operand stored as rows of
 // 128 bytes with the 128-byte swizzle (8-row atoms 1024 bytes apart).
 __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
