@@ -95,11 +95,17 @@ struct Cfg {
 };
 
 // K is walked in units of a stage (BS blocks; the last one may be shorter).
-// The cost of a split tail against a whole one, in 64-k blocks of a CTA's
-// time: publishing a partial tile, the ticket and the last arriver's sums.
+// The cost of a split tail against a whole one, in 64-k blocks: publishing a
+// partial tile, the ticket and the last arriver's sums. Measured, split against
+// whole, us: 16 rows, N = 28672: K = 4096 (28 blocks less on the longest CTA)
+// 21.2 / 19.7, K = 8192 (60 less) 32.0 / 33.6; N = K = 4096 (48) 13.2 / 11.0;
+// K = 14336, N = 4096 (172) 16.3 / 28.6. 64 rows: N = 28672, K = 8192 (60) 42.7 /
+// 41.2, N = K = 8192 (72) 21.8 / 22.4. 128 rows: N = 28672, K = 8192 (62) 68 / 61,
+// N = K = 8192 (72) 30.0 / 32.3. 256 rows, M = 1024: N = 20480, K = 4096 (43)
+// 129 / 127, N = 28672, K = 8192 (120) 300 / 320.
 template <int TILE_M>
 constexpr int split_overhead_blocks() {
-  return TILE_M <= 64 ? 24 : 36;
+  return TILE_M <= 32 ? 50 : (TILE_M <= 128 ? 70 : 48);
 }
 constexpr int kMinChunkBlocks = 8;
 constexpr int kMaxShares = 8;  // shares per tail tile on average
