@@ -17,10 +17,9 @@ from typing import NamedTuple
 
 import torch
 
-from . import (ACTIVATIONS, GROUP_SCORES, SCORINGS, Epilogue, RouteOptions,
-               experts_workspace_size, launch_quantize_repack, launch_repack_scales_128,
-               launch_repack_umma, route_workspace_size)
-from .launching import on, run, size, want, want_out, workspace
+from . import (ACTIVATIONS, GROUP_SCORES, SCORINGS, launch_quantize_repack,
+               launch_repack_scales_128, launch_repack_umma)
+from .launching import binding, cuda_device, on
 from .linear import interleave_gate_up
 
 
@@ -42,59 +41,22 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     sigmoid scores, ``bias`` (float32 [E]) added for the choice only, the best
     ``topk_group`` of ``n_group`` groups, ties to the lowest index, weights
     renormalised to sum 1 and scaled."""
-    if scoring not in SCORINGS or group_score not in GROUP_SCORES:
+    kind, of_group = SCORINGS.get(scoring), GROUP_SCORES.get(group_score)
+    if kind is None or of_group is None:
         raise ValueError(f"unknown scoring {scoring!r} or group_score {group_score!r}")
-    want(logits, "logits", (torch.float32, torch.float16))
-    if logits.dim() != 2:
-        raise ValueError("logits must be [T, E]")
-    T, E = logits.shape
-    dev = logits.device
+    dev = cuda_device(logits, "logits")
     with on(dev, stream, logits, bias):
-        if logits.stride(1) != 1 or logits.stride(0) < E:
-            logits = logits.contiguous()
-        if bias is not None:
-            bias = want(bias, "bias", torch.float32, (E,), dev).contiguous()
-        r = Routing(torch.empty(T, top_k, dtype=torch.int32, device=dev),
-                    torch.empty(T, top_k, dtype=torch.float32, device=dev),
-                    torch.empty(E + 1, dtype=torch.int32, device=dev),
-                    torch.empty(T * top_k, dtype=torch.int32, device=dev),
-                    torch.empty(T, top_k, dtype=torch.int32, device=dev))
-        options = RouteOptions(SCORINGS[scoring], n_group, topk_group, GROUP_SCORES[group_score],
-                               renormalize, scale)
-        need = size(route_workspace_size, dev, T, E)  # for its counts; nothing is kept in it
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        run("i4g_route", dev, logits.data_ptr(), logits.dtype == torch.float32,
-            logits.stride(0) if T > 1 else E, 0 if bias is None else bias.data_ptr(), T, E, top_k,
-            options, r.ids.data_ptr(), r.weights.data_ptr(), r.offsets.data_ptr(),
-            r.rows.data_ptr(), r.slots.data_ptr(), 0 if ws is None else ws.data_ptr(), need)
-    return r
+        return Routing(*binding().route(logits, top_k, kind, bias, n_group, topk_group, of_group,
+                                        renormalize, scale))
 
 
 def combine(y: torch.Tensor, routing: Routing, *, residual: torch.Tensor | None = None,
             out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t] = residual[t] + sum over places s of weights[t, s] * y[slots[t, s]]
     (C ABI i4g_experts_combine): y fp16 in expert order, out fp16 [T, N]."""
-    want(y, "y", torch.float16)
-    dev = y.device
-    weights, slots = routing.weights, routing.slots
-    T, top_k = slots.shape
-    want_out(slots, "routing.slots", torch.int32, (T, top_k), dev)
-    want_out(weights, "routing.weights", torch.float32, (T, top_k), dev)
-    if y.dim() != 2:
-        raise ValueError("y must be [rows, N]")
-    N = y.shape[1]
-    if out is not None:
-        want_out(out, "out", torch.float16, (T, N), dev)
-    with on(dev, stream, y, weights, slots, residual, out):
-        y = y.contiguous()
-        if residual is not None:
-            residual = want(residual, "residual", torch.float16, (T, N), dev).contiguous()
-        if out is None:
-            out = torch.empty(T, N, dtype=torch.float16, device=dev)
-        run("i4g_experts_combine", dev, y.data_ptr(), y.shape[0], slots.data_ptr(),
-            weights.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(), T,
-            top_k, N)
-    return out
+    dev = cuda_device(y, "y")
+    with on(dev, stream, y, routing.weights, routing.slots, residual, out):
+        return binding().combine(y, routing.slots, routing.weights, residual, out)
 
 
 class QuantizedExperts:
@@ -120,12 +82,12 @@ class QuantizedExperts:
     @classmethod
     def from_weight(cls, w: torch.Tensor, group: int, stream=None) -> "QuantizedExperts":
         """Quantise fp16 [E, K, N] weights, each as QuantizedLinear.from_weight does."""
-        want(w, "weight", torch.float16)
-        if w.dim() != 3:
-            raise ValueError("weight must be [E, K, N]")
+        dev = cuda_device(w, "weight")
+        if w.dtype != torch.float16 or w.dim() != 3:
+            raise TypeError("weight must be a 3-D float16 CUDA tensor [E, K, N]")
         E, K, N = w.shape
-        with on(w.device, stream, w):
-            self = cls._empty(E, K, N, group, w.device)
+        with on(dev, stream, w):
+            self = cls._empty(E, K, N, group, dev)
             for e in range(E):
                 launch_quantize_repack(w[e].contiguous(), self.tiles[e], self.scales[e], K, N,
                                        group)
@@ -142,9 +104,9 @@ class QuantizedExperts:
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, K: int, N: int, group: int,
                     stream=None) -> "QuantizedExperts":
         """Repack quantiser-layout codes [E][K * N / 2] and scales [E][K / group][N]."""
-        want(packed, "packed", torch.uint8)
-        E, dev = packed.shape[0], packed.device
-        want(scales, "scales", torch.float16, None, dev)
+        E, dev = packed.shape[0], cuda_device(packed, "packed")
+        if packed.dtype != torch.uint8 or scales.dtype != torch.float16 or scales.device != dev:
+            raise TypeError("packed must be uint8 and scales float16, on one device")
         if packed.numel() != E * (K * N // 2) or scales.numel() != E * (K // group) * N:
             raise ValueError("buffer sizes do not match E, K, N, group")
         with on(dev, stream, packed, scales):
@@ -163,35 +125,14 @@ class QuantizedExperts:
         gather: ``a`` is the tokens' rows [T, K]; otherwise rows already in
         expert order [T * top_k, K]. bias: fp16 [E, N]. Rows of the result past
         routing.offsets[E] are left as they were."""
-        if activation not in ACTIVATIONS:
+        kind = ACTIVATIONS.get(activation)
+        if kind is None:
             raise ValueError(f"unknown activation {activation!r}")
-        dev = self.tiles.device
-        want(a, "A", torch.float16, None, dev)
-        T, top_k = routing.slots.shape
-        pairs = T * top_k
-        want_out(routing.offsets, "routing.offsets", torch.int32, (self.E + 1,), dev)
-        want_out(routing.rows, "routing.rows", torch.int32, (pairs,), dev)
-        rows_a = T if gather else pairs
-        if a.dim() != 2 or a.shape[0] != rows_a or a.shape[1] != self.K:
-            raise ValueError(f"A must be float16 [{rows_a}, {self.K}]")
-        cols = self.N // 2 if gated else self.N
-        dtype = torch.float32 if fp32_out else torch.float16
-        if out is not None:
-            want_out(out, "out", dtype, (pairs, cols), dev)
+        dev = cuda_device(self.tiles, "the weights")
         with on(dev, stream, a, routing.offsets, routing.rows, bias, out):
-            a = a.contiguous()
-            if bias is not None:
-                bias = want(bias, "bias", torch.float16, (self.E, self.N), dev).contiguous()
-            if out is None:
-                out = torch.empty(pairs, cols, dtype=dtype, device=dev)
-            ws = workspace(size(experts_workspace_size, dev, pairs, self.E, self.N, self.K), dev)
-            e = Epilogue(0 if bias is None else bias.data_ptr(), 0, 0, ACTIVATIONS[activation],
-                         gated, fp32_out)
-            run("i4g_experts_gemm", dev, a.data_ptr(), rows_a, self.tiles.data_ptr(),
-                self.scales.data_ptr(), out.data_ptr(), routing.offsets.data_ptr(),
-                routing.rows.data_ptr() if gather else 0, top_k, pairs, self.E, self.N, self.K,
-                self.group, e, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-        return out
+            return binding().experts_gemm(a, self.tiles, self.scales, self.E, self.K, self.N,
+                                          self.group, routing.offsets, routing.rows,
+                                          routing.slots, gather, bias, kind, gated, out, fp32_out)
 
 
 class ExpertMLP:

@@ -9,10 +9,9 @@ from __future__ import annotations
 
 import torch
 
-from . import (ACTIVATIONS, Epilogue, gemm_epilogue_workspace_size, launch_final_fp32_ws,
-               launch_final_ws, launch_quantize_repack, launch_repack_scales_128,
-               launch_repack_umma, shard_range, workspace_for)
-from .launching import on, run, size, want, want_out, workspace
+from . import (ACTIVATIONS, launch_final_fp32_ws, launch_final_ws, launch_quantize_repack,
+               launch_repack_scales_128, launch_repack_umma, shard_range, workspace_for)
+from .launching import binding, cuda_device, on
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -99,33 +98,10 @@ class QuantizedLinear:
         return out
 
     def _epilogue(self, a, out, fp32_out, stream, bias, activation, gated, residual):
-        if activation not in ACTIVATIONS:
+        kind = ACTIVATIONS.get(activation)
+        if kind is None:
             raise ValueError(f"unknown activation {activation!r}")
-        dev = self.tiles.device
-        want(a, "A", torch.float16, None, dev)
-        if a.dim() != 2 or a.shape[1] != self.K:
-            raise ValueError(f"A must be float16 [M, {self.K}]")
-        M, cols = a.shape[0], self.N // 2 if gated else self.N
-        dtype = torch.float32 if fp32_out else torch.float16
-        if out is not None:
-            want_out(out, "out", dtype, (M, cols), dev)
+        dev = cuda_device(self.tiles, "the weight")
         with on(dev, stream, a, bias, residual, out):
-            a = a.contiguous()
-            ld = 0
-            if bias is not None:
-                bias = want(bias, "bias", torch.float16, (self.N,), dev).contiguous()
-            if residual is not None:
-                want(residual, "residual", torch.float16, (M, cols), dev)
-                if residual.stride(1) != 1 or residual.stride(0) < cols:
-                    residual = residual.contiguous()
-                ld = residual.stride(0)
-            if out is None:
-                out = torch.empty(M, cols, dtype=dtype, device=dev)
-            ws = workspace(size(gemm_epilogue_workspace_size, dev, M, self.N, self.K), dev)
-            e = Epilogue(0 if bias is None else bias.data_ptr(),
-                         0 if residual is None else residual.data_ptr(), ld,
-                         ACTIVATIONS[activation], gated, fp32_out)
-            run("i4g_gemm_epilogue", dev, a.data_ptr(), self.tiles.data_ptr(),
-                self.scales.data_ptr(), out.data_ptr(), M, self.N, self.K, self.group, e,
-                0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-        return out
+            return binding().gemm_epilogue(a, self.tiles, self.scales, self.K, self.N, self.group,
+                                           bias, kind, gated, residual, out, fp32_out)
