@@ -377,6 +377,18 @@ int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scal
     return fail(I4G_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != I4G_OK) return st;
+  if (!offsets && i4g::epi::decode_is_faster(M, N, K, dev->sm_count)) {
+    CUtensorMap dmap;
+    if ((st = epi_map(A, M, K, i4g::dec::rows_for(M), 4, &dmap)) != I4G_OK) return st;
+    const i4g::EpilogueOut out{C, e.gated ? N / 2 : N, e.fp32_out, e.gated,
+                               i4g::Epilogue{static_cast<const __half*>(e.bias),
+                                             static_cast<const __half*>(e.residual),
+                                             e.ld_residual, e.activation}};
+    return finish(i4g::dec::launch_epilogue(dmap, tiles, static_cast<const __half*>(scales), out,
+                                            M, N, K, group, dev->sm_count, dev->status_word,
+                                            g_wait_limit_ns, static_cast<cudaStream_t>(stream)),
+                  "decode kernel launch");
+  }
   const int tile_m = i4g::epi::choose_tile(offsets ? mean_rows(M, E) : M);
   const long tiles_most = i4g::epi::tiles_bound(tile_m, M, E, N);
   // the workspace holds the split tail's part, then the activations in row
@@ -775,6 +787,7 @@ int i4g_gemm_epilogue_workspace_size(int M, int N, int K, size_t* bytes) {
   if (M == 0) return I4G_OK;
   DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != I4G_OK) return st;
+  if (i4g::epi::decode_is_faster(M, N, K, dev->sm_count)) return I4G_OK;  // needs none
   const int tile_m = i4g::epi::choose_tile(M);
   *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, M, 1, N), K,
                                      dev->sm_count);

@@ -24,6 +24,13 @@ struct Epilogue {
   int activation;
 };
 
+// Where the decode kernel puts the results: one contiguous matrix.
+struct EpilogueOut {
+  void* C;       // [M][ldc], half or float
+  int ldc, fp32_out, gated;
+  Epilogue epilogue;
+};
+
 // x * sigmoid(x (c0 + c1 x^2)): SiLU is c0 = 1, c1 = 0; tanh-GELU, whose
 // 0.5 (1 + tanh(u / 2)) is sigmoid(u), is c0 = sqrt(8/pi), c1 = 0.044715 c0.
 // 1 + exp(-u) overflows to infinity for very negative u and the quotient is

@@ -26,6 +26,7 @@
 // (deterministic, no global scratch).
 #include "ptx.cuh"
 #include "gemm_tc.h"
+#include "epilogue.cuh"
 
 #include <cuda_runtime.h>
 
@@ -348,11 +349,52 @@ __device__ __forceinline__ void store_fragment(const Outputs& out, int M, int nt
   }
 }
 
-template <int MT, int GROUP, int STAGES>
+// The same fragment through the fused epilogue (epilogue.cuh): a gate (x, y)
+// and the column it gates (z, w) are the lane's two columns, 8 apart.
+__device__ __forceinline__ void store_fragment(const EpilogueOut& out, int M, int nt, int w,
+                                               int ln, int mb, float4 v) {
+  const int col = nt * NCOL + w * 16 + (ln >> 2);
+  const int m = mb * 8 + 2 * (ln & 3);
+  const Epilogue& e = out.epilogue;
+  if (e.bias) {
+    const float b0 = __half2float(e.bias[col]), b1 = __half2float(e.bias[col + 8]);
+    v.x += b0;
+    v.y += b0;
+    v.z += b1;
+    v.w += b1;
+  }
+  auto put = [&](int row, int c, float y) {
+    if (row >= M) return;
+    if (e.residual) y += __half2float(e.residual[static_cast<size_t>(row) * e.ldr + c]);
+    const size_t at = static_cast<size_t>(row) * out.ldc + c;
+    if (out.fp32_out) static_cast<float*>(out.C)[at] = y;
+    else static_cast<__half*>(out.C)[at] = __float2half_rn(y);
+  };
+  if (out.gated) {
+    float g[2] = {v.x, v.y};
+    activate(e.activation, g);
+    const int c = nt * (NCOL / 2) + w * 8 + (ln >> 2);
+    put(m, c, g[0] * v.z);
+    put(m + 1, c, g[1] * v.w);
+  } else {
+    float y[4] = {v.x, v.y, v.z, v.w};
+    activate(e.activation, y);
+    put(m, col, y[0]);
+    put(m + 1, col, y[1]);
+    put(m, col + 8, y[2]);
+    put(m + 1, col + 8, y[3]);
+  }
+}
+
+// Copies of C beyond this GPU's are read by other GPUs.
+__device__ __forceinline__ bool has_peers(const Outputs& out) { return out.count > 1; }
+__device__ __forceinline__ bool has_peers(const EpilogueOut&) { return false; }
+
+template <int MT, int GROUP, int STAGES, typename Out>
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     decode_kernel(const __grid_constant__ CUtensorMap act_map,
                   const uint8_t* __restrict__ tiles, const __half* __restrict__ scales,
-                  const __grid_constant__ Outputs out, int M, int N, int K, int* status,
+                  const __grid_constant__ Out out, int M, int N, int K, int* status,
                   unsigned long long wait_limit_ns, int prefetch_blocks) {
   using L = Layout<MT, GROUP, STAGES>;
   extern __shared__ uint8_t smem_raw[];
@@ -491,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     const int th = x / MT;
     store_fragment(out, M, nt, th >> 5, th & 31, x % MT, sum);
   }
-  if (out.count > 1) __threadfence_system();  // peer copies are read by other GPUs
+  if (has_peers(out)) __threadfence_system();  // peer copies are read by other GPUs
   cluster_sync();  // every CTA's shared memory stays alive until all have read it
 }
 
@@ -986,13 +1028,13 @@ int prefetch_blocks() {
   return v;
 }
 
-template <int MT, int GROUP>
+template <int MT, int GROUP, typename Out>
 cudaError_t launch_typed(const CUtensorMap& act_map, const uint8_t* tiles, const __half* scales,
-                         const Outputs& out, int M, int N, int K, int cluster, bool pdl,
+                         const Out& out, int M, int N, int K, int cluster, bool pdl,
                          int* status, unsigned long long wait_limit_ns, cudaStream_t stream) {
   constexpr int S = stages_for<MT, GROUP>();
   using L = Layout<MT, GROUP, S>;
-  auto kernel = decode_kernel<MT, GROUP, S>;
+  auto kernel = decode_kernel<MT, GROUP, S, Out>;
   static std::atomic<uint64_t> configured{0};  // devices set, per instantiation
   cudaError_t e = ensure_dynamic_smem(kernel, L::DYN, configured);
   if (e != cudaSuccess) return e;
@@ -1207,7 +1249,7 @@ template <int MT, int GROUP>
 cudaError_t resources_of(KernelResources* out) {
   constexpr int S = stages_for<MT, GROUP>();
   using L = Layout<MT, GROUP, S>;
-  auto kernel = decode_kernel<MT, GROUP, S>;
+  auto kernel = decode_kernel<MT, GROUP, S, Outputs>;
   static std::atomic<uint64_t> configured{0};
   cudaError_t e = ensure_dynamic_smem(kernel, L::DYN, configured);
   if (e != cudaSuccess) return e;
@@ -1292,6 +1334,23 @@ cudaError_t launch(const CUtensorMap& act_map, const __half* A, const uint8_t* t
                         use_sk ? &sk : nullptr, workspace, status, wait_limit_ns, stream);
   return launch_mt<2>(act_map, tiles, scales, out, M, N, K, group, cluster, pdl,
                       use_sk ? &sk : nullptr, workspace, status, wait_limit_ns, stream);
+}
+
+cudaError_t launch_epilogue(const CUtensorMap& act_map, const uint8_t* tiles,
+                            const __half* scales, const EpilogueOut& out, int M, int N, int K,
+                            int group, int sm_count, int* status,
+                            unsigned long long wait_limit_ns, cudaStream_t stream) {
+  const int cluster = choose_cluster(N, K, sm_count);
+  const int free_slots = CTAS_PER_SM * sm_count - (N / NCOL) * cluster;
+  const bool pdl = pdl_enabled() && free_slots >= kPdlFreeSlots;
+#define I4G_DEC_EPI(MT, G)                                                                    \
+  if (M <= MT * 8 && group == G)                                                              \
+    return launch_typed<MT, G>(act_map, tiles, scales, out, M, N, K, cluster, pdl, status,    \
+                               wait_limit_ns, stream);
+  I4G_DEC_EPI(1, 32) I4G_DEC_EPI(1, 64) I4G_DEC_EPI(1, 128)
+  I4G_DEC_EPI(2, 32) I4G_DEC_EPI(2, 64) I4G_DEC_EPI(2, 128)
+#undef I4G_DEC_EPI
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace dec

@@ -38,6 +38,8 @@ struct Sched {
 
 // Activation rows per tile for `rows` rows per weight (16, 32, 64, 128, 256).
 int choose_tile(int rows);
+// Whether the decode kernel's cluster schedule serves a dense product faster.
+bool decode_is_faster(int M, int N, int K, int sm_count);
 // Rows of a tile from which gathered activations are first copied into row
 // order by a kernel of their own (gather_rows) instead of four rows per copy
 // instruction inside the product.

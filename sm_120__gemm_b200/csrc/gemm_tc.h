@@ -10,6 +10,8 @@
 
 namespace i4g {
 
+struct EpilogueOut;  // epilogue.cuh
+
 // Raises `kernel`'s dynamic shared-memory limit to `bytes` on the current
 // device, once per device: the attribute belongs to the kernel's instance on
 // each device, so a process that drives several GPUs sets it on every one.
@@ -146,6 +148,12 @@ cudaError_t launch(const CUtensorMap& act_map, const __half* A, const uint8_t* t
                    const __half* scales, const Outputs& out, int M, int N, int K, int group,
                    int sm_count, void* workspace, size_t workspace_bytes, int* status,
                    unsigned long long wait_limit_ns, cudaStream_t stream);
+// The cluster schedule with the fused epilogue (M <= MAX_M; no workspace).
+// act_map: rows_for(M) rows x four 64-k blocks a box.
+cudaError_t launch_epilogue(const CUtensorMap& act_map, const uint8_t* tiles,
+                            const __half* scales, const EpilogueOut& out, int M, int N, int K,
+                            int group, int sm_count, int* status,
+                            unsigned long long wait_limit_ns, cudaStream_t stream);
 }  // namespace dec
 
 namespace prep {

@@ -62,8 +62,10 @@ def test_groups_and_types(i4g, group, M, fp32):
     run(i4g, M, 256, 384, group, "gelu", gated=(group == 64), bias=True, residual=True, fp32=fp32)
 
 
-# tails cut along K: few tiles and long K, more tiles than SMs, promotion
+# tails cut along K: few tiles and long K, more tiles than SMs, promotion; up to
+# 16 rows both kernels that serve them
 @pytest.mark.parametrize("M,N,K", [(1, 128, 14336), (7, 256, 8192), (1, 28672, 2048),
+                                   (3, 28672, 8192), (13, 20480, 4160), (16, 57344, 1024),
                                    (40, 4096, 8192), (64, 128, 6144 + 64), (100, 640, 8192),
                                    (300, 640, 8192), (520, 7168, 4160), (1024, 2048, 12288)])
 @pytest.mark.parametrize("gated", [False, True])
@@ -71,8 +73,8 @@ def test_split_tails(i4g, M, N, K, gated):
     run(i4g, M, N, K, 64, "silu" if gated else "none", gated, bias=True, residual=True)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 28672, 2048), (40, 4096, 8192), (100, 640, 8192),
-                                   (300, 640, 8192), (1024, 3200, 12288), (520, 7168, 4160)])
+@pytest.mark.parametrize("M,N,K", [(1, 28672, 2048), (3, 28672, 8192), (40, 4096, 8192),
+                                   (100, 640, 8192), (300, 640, 8192), (1024, 3200, 12288), (520, 7168, 4160)])
 def test_split_tails_repeat_bit_for_bit(i4g, M, N, K):
     lin, _ = make(i4g, K, N, 64)
     a = rand(M, K, seed=9)
@@ -155,6 +157,7 @@ def test_empty_batch_and_refusals(i4g):
 
 def test_workspace_none_small_and_enough_agree(i4g):
     M, N, K = 24, 512, 8192
+    assert i4g.gemm_epilogue_workspace_size(4, N, K) == 0  # the decode kernel
     lin, w64 = make(i4g, K, N, 64)
     a = rand(M, K, seed=3)
     need = i4g.gemm_epilogue_workspace_size(M, N, K)
@@ -174,7 +177,8 @@ def test_workspace_none_small_and_enough_agree(i4g):
 def test_graphs_share_nothing(i4g):
     """Two captured graphs replayed on two streams at once, and eager calls
     between: every result as if run alone."""
-    M, N, K = 8, 1024, 8192
+    M, N, K = 24, 1024, 8192
+    assert i4g.gemm_epilogue_workspace_size(M, N, K) > 0
     lin, _ = make(i4g, K, N, 128)
     a = [rand(M, K, seed=20 + i) for i in range(3)]
     want = [lin(x, activation="silu", gated=True) for x in a]

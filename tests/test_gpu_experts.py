@@ -285,6 +285,35 @@ def test_combine_skips_and_in_place(i4g):
         i4g.combine(rand(6, 12), r)
 
 
+def test_launch_functions(i4g):
+    """The C ABI's Python mirrors, as a caller with its own buffers uses them."""
+    T, E, k, K, N, g = 9, 6, 2, 128, 128, 64
+    ex = i4g.QuantizedExperts.from_weight(rand(E, K, N, seed=1, scale=0.05), g)
+    x = rand(T, K, seed=2)
+    logits = rand(T, E, seed=3, dtype=torch.float32)
+    want = i4g.route(logits, k, scoring="sigmoid", scale=0.5)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    r = i4g.Routing(torch.empty(T, k, **i32), torch.empty(T, k, device="cuda"),
+                    torch.empty(E + 1, **i32), torch.empty(T * k, **i32),
+                    torch.empty(T, k, **i32))
+    assert i4g.route_workspace_size(T, E) == 0 and i4g.route_workspace_size(5000, E) > 0
+    options = i4g.RouteOptions(i4g.SCORINGS["sigmoid"], 1, 1, i4g.GROUP_SCORES["max"], 1, 0.5)
+    i4g.launch_route(logits, True, E, None, T, E, k, options, *r)
+    for p, q in zip(r, want):
+        assert torch.equal(p, q)
+    y = torch.empty(T * k, N, dtype=torch.float16, device="cuda")
+    ws = torch.zeros(max(256, i4g.experts_workspace_size(T * k, E, N, K)), dtype=torch.uint8,
+                     device="cuda")
+    i4g.launch_experts(x, T, ex.tiles, ex.scales, y, r.offsets, r.rows, k, T * k, E, N, K, g,
+                       activation="relu", workspace=ws)
+    assert torch.equal(y, ex(x, want, activation="relu"))
+    out = torch.empty(T, N, dtype=torch.float16, device="cuda")
+    i4g.launch_combine(y, T * k, r.slots, r.weights, None, out, T, k, N)
+    assert torch.equal(out, i4g.combine(y, want))
+    with pytest.raises(i4g.I4GError):
+        i4g.launch_route(logits, True, E, None, 5000, E, k, options, *r)  # no workspace
+
+
 def plain_moe(x, logits, k, wg, wu, wd, group, act, residual, **route_kw):
     """The block in 64 bits, rounded to fp16 where the block rounds."""
     ids, w, *_ = ref.route(logits, k, **route_kw)
