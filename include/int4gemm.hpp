@@ -124,6 +124,43 @@ inline void launch_final_fp32_ws(const half* a, const uint8_t* b, const half* s,
       "launch_final_fp32_ws");
 }
 
+// New: launch_final with bias, activation (or gate) and residual fused into
+// the epilogue; c is half or, with e.fp32_out, float.
+inline void launch_final_epilogue(const half* a, const uint8_t* b, const half* s, void* c, int M,
+                                  int N, int K, int group, const i4g_epilogue_t& e,
+                                  void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  i4g_throw_if(i4g_gemm_epilogue(a, b, s, c, M, N, K, group, &e, workspace, workspace_bytes,
+                                 stream),
+               "launch_final_epilogue");
+}
+
+// New: a mixture of experts over INT4 weights (i4g.h): routing, the experts'
+// products over the sorted rows, and their combination.
+inline void launch_route(const void* logits, bool fp32_logits, int ld_logits, const float* bias,
+                         int T, int E, int top_k, const i4g_route_t& options, int32_t* ids,
+                         float* weights, int32_t* offsets, int32_t* rows, int32_t* slots,
+                         void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  i4g_throw_if(i4g_route(logits, fp32_logits, ld_logits, bias, T, E, top_k, &options, ids,
+                         weights, offsets, rows, slots, workspace, workspace_bytes, stream),
+               "launch_route");
+}
+
+inline void launch_experts(const half* a, int a_rows, const uint8_t* b, const half* s, void* c,
+                           const int32_t* offsets, const int32_t* rows, int row_div, int pairs,
+                           int E, int N, int K, int group, const i4g_epilogue_t& e,
+                           void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  i4g_throw_if(i4g_experts_gemm(a, a_rows, b, s, c, offsets, rows, row_div, pairs, E, N, K, group,
+                                &e, workspace, workspace_bytes, stream),
+               "launch_experts");
+}
+
+inline void launch_combine(const half* y, int y_rows, const int32_t* slots, const float* weights,
+                           const half* residual, half* out, int T, int top_k, int N,
+                           cudaStream_t stream) {
+  i4g_throw_if(i4g_experts_combine(y, y_rows, slots, weights, residual, out, T, top_k, N, stream),
+               "launch_combine");
+}
+
 inline void launch_final(const half* a, const uint8_t* b, const half* s, half* c, int M, int N,
                          int K, int group, cudaStream_t stream) {
   i4g_throw_if(i4g_gemm(a, b, s, c, M, N, K, group, stream), "launch_final");

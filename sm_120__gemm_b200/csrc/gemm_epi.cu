@@ -14,17 +14,18 @@ int choose_tile(int rows) {
 
 // Both kernels' times in us, as lines through measurements on B200 (back-to-back
 // calls, g128): each in the 64-k blocks of its busiest SM. Decode / this kernel
-// at M = 8: N = K = 4096 7.1 / 11.0; K = 14336, N = 4096 12.9 / 16.3; K = 4096,
-// N = 14336 13.5 / 13.5, N = 28672 21.4 / 19.7; K = 8192, N = 28672 37 / 32; at
+// at M = 8: N = K = 4096 5.5 / 11.0; K = 14336, N = 4096 11.2 / 16.3; K = 4096,
+// N = 14336 11.4 / 13.4, N = 28672 19.2 / 19.5; K = 8192, N = 28672 35 / 32. At
 // M = 16 the decode kernel's second row of fragments costs it a quarter more
-// (26.2 / 19.7 and 45.7 / 32 for the last two).
+// (K = 4096, N = 14336 13.8 / 13.4, N = 28672 24 / 19.5).
 bool decode_is_faster(int M, int N, int K, int sm_count) {
   if (M > dec::MAX_M) return false;
   const int kblocks = K / BK;
   const long tiles = N / TILE_N;
   const int cluster = dec::choose_cluster(N, K, sm_count);
   const long ctas = (tiles * cluster + sm_count - 1) / sm_count;  // of the busiest SM
-  const double decode = 5.2 + (M <= 8 ? 0.127 : 0.16) * ctas * ((kblocks + cluster - 1) / cluster);
+  const long blocks = ctas * ((kblocks + cluster - 1) / cluster);
+  const double decode = M <= 8 ? 3.9 + 0.1185 * blocks : 4.2 + 0.15 * blocks;
   using L = Cfg<16>;
   const int kunits = (kblocks + L::BS - 1) / L::BS;
   const Sched s = make_sched(static_cast<int>(tiles), kunits, L::BS, sm_count, true,

@@ -29,7 +29,7 @@ cudaError_t ensure_dynamic_smem(Kernel kernel, int bytes, std::atomic<uint64_t>&
   return e;
 }
 
-// The GEMM kernels are launched as programmatic dependents of the kernel
+// The kernels of a step are launched as programmatic dependents of the kernel
 // before them on the stream (they may start while it runs, and wait for it
 // before touching A, C or a workspace), unless I4G_PDL=0 (read once).
 inline bool pdl_enabled() {

@@ -26,6 +26,7 @@
 // maximum of order-preserving integer keys and a ballot.
 #include "route.h"
 
+#include "gemm_tc.h"
 #include "ptx.cuh"
 
 #include <algorithm>
@@ -558,7 +559,7 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), int grid, int threads, cu
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -666,7 +667,7 @@ cudaError_t combine(const __half* y, int y_rows, const int* slots, const float* 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, combine_kernel, y, y_rows, slots, weights, residual, out, top_k,
                             N);
 }

@@ -178,6 +178,41 @@ def test_interleave_gate_up(m):
         interleave_gate_up(gate, up[:1])
 
 
+def test_cpp_wrappers_throw(tmp_path):
+    """The C++ forms compile and turn a refusal into std::runtime_error."""
+    import os
+    import shutil
+    import subprocess
+
+    from conftest import ROOT
+    if shutil.which("g++") is None:
+        pytest.skip("no host C++ compiler")
+    src = tmp_path / "t.cpp"
+    src.write_text(r'''
+#include "int4gemm.hpp"
+#include <cstdio>
+template <typename F> int throws(F f) {
+  try { f(); } catch (const std::runtime_error& e) { std::printf("%s\n", e.what()); return 1; }
+  return 0;
+}
+int main() {
+  using namespace int4gemm;
+  i4g_epilogue_t e{};
+  i4g_route_t r{I4G_SCORE_SOFTMAX, 1, 1, I4G_GROUP_MAX, 1, 1.0f};
+  return 4 - throws([&] { launch_final_epilogue(0, 0, 0, 0, 4, 100, 128, 64, e, 0, 0, 0); }) -
+         throws([&] { launch_route(0, true, 8, 0, 4, 8, 9, r, 0, 0, 0, 0, 0, 0, 0, 0); }) -
+         throws([&] { launch_experts(0, 4, 0, 0, 0, 0, 0, 0, 8, 2, 128, 128, 48, e, 0, 0, 0); }) -
+         throws([&] { launch_combine(0, 8, 0, 0, 0, 0, 4, 2, 12, 0); });
+}
+''')
+    pkg = os.path.join(ROOT, "sm_120__gemm_b200")
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "include"), "-I",
+                    "/usr/local/cuda/include", str(src), "-o", str(tmp_path / "t"), "-L", pkg,
+                    "-li4g", f"-Wl,-rpath,{pkg}"], check=True)
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True)
+    assert out.returncode == 0, out
+
+
 def test_plain_routing_of_a_worked_example():
     """The checker itself, on numbers worked by hand."""
     import operators_ref as ref
