@@ -45,8 +45,8 @@ __device__ __forceinline__ float sigmoid_gate(float x, float c0, float c1) {
 // cancellation on the negative side. erfc(z) exp(z^2) is a polynomial of degree
 // 8 in t = 1 / (1 + z / 2), times t, fitted by weighted least squares for the
 // least largest relative error (4e-8; 3.3e-7 evaluated in FP32): 20
-// instructions, where the library's erfc cost 8 us of a 42 us product (M = 203,
-// N = 14336, whose one wave of tiles hides no epilogue).
+// instructions (M = 203, N = 14336, whose one wave of tiles hides no epilogue:
+// 36.2 us, and 41.6 with the library's erfc).
 __device__ __forceinline__ float gelu_erf(float x) {
   const float a = fminf(fabsf(x), 40.0f);  // exp(-800) is 0: infinities keep their limits
   const float t = __fdividef(1.0f, fmaf(a, 0.35355339f, 1.0f));

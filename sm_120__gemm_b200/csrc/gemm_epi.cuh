@@ -53,7 +53,7 @@ constexpr int kTableInts = kMaxExperts + 1 + 32;
 
 template <int TILE_M>
 struct Cfg {
-    static constexpr int DEQ = TILE_M <= 128 ? 3 : 1;  // dequant groups
+  static constexpr int DEQ = TILE_M <= 128 ? 3 : 1;  // dequant groups
   static constexpr int PARTS = TILE_M <= 32 ? 1 : (TILE_M <= 128 ? 2 : 4);
   static constexpr int EPI_WARPS = 4 * PARTS;
   static constexpr int COLS = TILE_M / PARTS;  // accumulator columns per epilogue thread
