@@ -47,13 +47,20 @@ constexpr int BK = 64;
 constexpr int T_COLS = 32;                     // TMEM columns per weight stage
 constexpr int TMEM_COLS = 512;
 constexpr int WBLOCK_BYTES = TILE_N * BK / 2;  // 4096
-constexpr int FIRST_DEQ_WARP = 3;
 constexpr int kPromoteBlocks = 32;             // 2048 k, as gemm_tc.cu
 constexpr int kTableInts = kMaxExperts + 1 + 32;
 
 template <int TILE_M>
 struct Cfg {
-  static constexpr int DEQ = TILE_M <= 128 ? 3 : 1;  // dequant groups
+  static constexpr int DEQ = TILE_M <= 128 ? 3 : 2;  // dequant groups
+  // At 256 rows 28 warps share the registers: launched with 72 each, the warps
+  // that only issue copies and MMAs hand theirs to the epilogue, which holds 64
+  // sums a thread (a scheduler's seven warps: 40 + 2 x 64 + 4 x 80 <= 7 x 72).
+  // With one group, 23 warps and no such split, M = 160, K = 4096, N = 14336
+  // took 28.6 us instead of 23.9, M = 4096, N = 28672 740 instead of 720; three
+  // groups were no faster.
+  static constexpr bool SPLIT_REGS = TILE_M == 256;
+  static constexpr int FIRST_DEQ_WARP = SPLIT_REGS ? 4 : 3;  // a split is by whole warpgroups
   static constexpr int PARTS = TILE_M <= 32 ? 1 : (TILE_M <= 128 ? 2 : 4);
   static constexpr int EPI_WARPS = 4 * PARTS;
   static constexpr int COLS = TILE_M / PARTS;  // accumulator columns per epilogue thread
@@ -406,175 +413,179 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     walk.start();
   }
 
-  if (warp == 0) {
-    // ------------------------------------------------- activation producer
-    // Gathered rows: lane l fetches rows 4 l .. 4 l + 3 of the tile (and 128
-    // further where the tile has them) while there are any; the last fetch may
-    // repeat the tile's last row. Rows that are not fetched keep what the
-    // stage held: each belongs to one accumulator column, which is not stored.
-    constexpr int PER_LANE = (TILE_M / 4 + 31) / 32;
-    uint32_t it = 0, s = 0, ph = 0;
-    bool ok = true;
-    Item w;
-    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
-      int src[PER_LANE][4];
-      if (a.rows) {
-#pragma unroll
-        for (int q = 0; q < PER_LANE; ++q)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = min((lane + 32 * q) * 4 + i, w.rows - 1);
-            src[q][i] = a.rows[w.row0 + r] / a.row_div;
-          }
-      }
-      const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
-      const int row0 = static_cast<int>(uniform(w.row0));
-      const int quads = static_cast<int>(uniform((w.rows + 3) / 4));
-      for (int u = u0; u < u1; ++u) {
-        ok = mbar_wait_warp(empty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
-        if (!ok) break;
-        const uint32_t dst = act_base + s * L::ACT_BYTES;
-        if (!a.rows) {
-          // a box past the last block (in the last unit, if K / 64 is not a
-          // multiple of BS) reads zeros and counts its bytes like any other
-          if (elect_one()) {
-            mbar_arrive_expect_tx(full(s), L::ACT_BYTES);
-            tma_load_3d(dst, &act_map, full(s), 0, row0, u * L::BS);
-          }
-        } else {
-          const int nb = min(L::BS, kblocks - u * L::BS);
-          if (elect_one()) mbar_arrive_expect_tx(full(s), nb * quads * 512);
-          __syncwarp();
-          for (int b = 0; b < nb; ++b)
-#pragma unroll
-            for (int q = 0; q < PER_LANE; ++q)
-              if (lane + 32 * q < quads)
-                tma_gather4(dst + b * L::BOX_BYTES + (lane + 32 * q) * 512, &act_map, full(s),
-                            (u * L::BS + b) * BK, src[q][0], src[q][1], src[q][2], src[q][3]);
+  if (warp < L::FIRST_DEQ_WARP) {
+    if constexpr (L::SPLIT_REGS) regs_dec<40>();
+    if (warp == 0) {
+      // ------------------------------------------------- activation producer
+      // Gathered rows: lane l fetches rows 4 l .. 4 l + 3 of the tile (and 128
+      // further where the tile has them) while there are any; the last fetch may
+      // repeat the tile's last row. Rows that are not fetched keep what the
+      // stage held: each belongs to one accumulator column, which is not stored.
+      constexpr int PER_LANE = (TILE_M / 4 + 31) / 32;
+      uint32_t it = 0, s = 0, ph = 0;
+      bool ok = true;
+      Item w;
+      for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
+        int src[PER_LANE][4];
+        if (a.rows) {
+  #pragma unroll
+          for (int q = 0; q < PER_LANE; ++q)
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = min((lane + 32 * q) * 4 + i, w.rows - 1);
+              src[q][i] = a.rows[w.row0 + r] / a.row_div;
+            }
         }
-        ++it;
-        if (++s == static_cast<uint32_t>(STAGES)) {
-          s = 0;
-          ph ^= 1u;
-        }
-      }
-    }
-    if (!ok && lane == 0) {  // let every copy already issued land
-      for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-        mbar_wait(full(i % STAGES), (i / STAGES) & 1u, never, nullptr, 100000000ull);
-    }
-  } else if (warp == 2) {
-    // ----------------------------------------------------- weight producer
-    uint32_t s = 0, ph = 0, issued = 0;
-    bool ok = true;
-    Item w;
-    for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
-      const size_t col = uniform(static_cast<uint32_t>(w.e * num_n + w.nt));  // 128-column run
-      const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
-      const int kb0 = u0 * L::BS;
-      const uint8_t* wsrc = a.tiles + (col * kblocks + kb0) * WBLOCK_BYTES;
-      const __half* ssrc = a.scales + (col * groups + kb0 * BK / GROUP) * TILE_N;
-      for (int u = u0; u < u1; ++u) {
-        ok = mbar_wait_warp(wempty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
-        if (!ok) break;
-        // a whole unit's sizes are constants; one that starts inside a group
-        // of 128 (one block a unit) still needs that group
-        constexpr uint32_t kGroupsFull = (L::BS * BK + GROUP - 1) / GROUP;
-        uint32_t wbytes = L::BS * WBLOCK_BYTES, sbytes = kGroupsFull * TILE_N * 2;
-        if (L::BS > 1 && u == kunits - 1) {
-          const uint32_t nb = kblocks - u * L::BS;
-          wbytes = nb * WBLOCK_BYTES;
-          sbytes = (nb * BK + GROUP - 1) / GROUP * TILE_N * 2;
-        }
-        if (elect_one()) {
-          const uint32_t dst = w_base + s * L::W_SLOT;
-          mbar_arrive_expect_tx(wfull(s), wbytes + sbytes);
-          bulk_load(dst, wsrc, wbytes, wfull(s));
-          bulk_load(dst + L::BS * WBLOCK_BYTES, ssrc, sbytes, wfull(s));
-        }
-        wsrc += L::BS * WBLOCK_BYTES;
-        if (L::BS * BK >= GROUP || (u & 1)) ssrc += kGroupsFull * TILE_N;
-        ++issued;
-        if (++s == static_cast<uint32_t>(W_STAGES)) {
-          s = 0;
-          ph ^= 1u;
-        }
-      }
-    }
-    if (!ok && lane == 0) {  // let every copy already issued land
-      for (uint32_t i = issued > W_STAGES ? issued - W_STAGES : 0; i < issued; ++i)
-        mbar_wait(wfull(i % W_STAGES), (i / W_STAGES) & 1u, never, nullptr, 100000000ull);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------- MMA issue
-    // Every loop bound is warp-uniform (see elect_one, uniform). The MMAs of a
-    // tall tile are as wide as its rows (rounded up to 16); below 64 rows the
-    // width costs no time and finding the rows would.
-    const uint64_t b_desc0 = smem_desc_sw128(act_base);
-    uint32_t s = 0, ph = 0;
-    uint32_t used[2] = {0, 0};  // segments committed per accumulator
-    int acc = 0;
-    bool ok = true;
-    Item w;
-    for (int j = 0; ok; ++j) {
-      uint32_t idesc = idesc_f16_f32(TILE_N, TILE_M);
-      if constexpr (TILE_M > 64) {
-        if (!__any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w))) break;
-        idesc = idesc_f16_f32(TILE_N, static_cast<int>(uniform((w.rows + 15) & ~15)));
-      } else {
-        if (!__any_sync(0xffffffffu, span_at(walk, j, w.u0, w.u1))) break;
-      }
-      const int u1 = static_cast<int>(uniform(w.u1));
-      int u = static_cast<int>(uniform(w.u0));
-      const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
-      uint32_t accumulate = 0;  // the item's first MMA starts the sum
-      while (true) {
-        // one segment of at most kPromoteBlocks blocks, once the accumulator
-        // is free: the last item drained it, or the epilogue promoted it
-        const uint32_t n = acc == 0 ? used[0]++ : used[1]++;
-        ok = mbar_wait_warp(dempty(acc), (n & 1u) ^ 1u, abort_flag, a.status, a.wait_limit_ns);
-        if (!ok) break;
-        tc_fence_after();
-        const int end = min(u1, u + kPromoteBlocks / L::BS);
-        for (; u < end; ++u) {
-          ok = mbar_wait_warp(full(s), ph, abort_flag, a.status, a.wait_limit_ns);
+        const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
+        const int row0 = static_cast<int>(uniform(w.row0));
+        const int quads = static_cast<int>(uniform((w.rows + 3) / 4));
+        for (int u = u0; u < u1; ++u) {
+          ok = mbar_wait_warp(empty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
           if (!ok) break;
-          tc_fence_after();
-          const uint64_t b_desc = b_desc0 + ((s * L::ACT_BYTES) >> 4);
-          const uint32_t a_tmem = tmem_base + s * L::T_STAGE;
-          if (u * L::BS + L::BS <= kblocks) {
-            if constexpr (L::BS == 4)
-              mma_f16_ts_blocks4(d_tmem, a_tmem, b_desc, idesc, accumulate, L::BOX_BYTES >> 4,
-                                 empty(s));
-            else if constexpr (L::BS == 2)
-              mma_f16_ts_blocks2(d_tmem, a_tmem, b_desc, idesc, accumulate, L::BOX_BYTES >> 4,
-                                 empty(s));
-            else
-              mma_f16_ts_blocks1(d_tmem, a_tmem, b_desc, idesc, accumulate, empty(s));
+          const uint32_t dst = act_base + s * L::ACT_BYTES;
+          if (!a.rows) {
+            // a box past the last block (in the last unit, if K / 64 is not a
+            // multiple of BS) reads zeros and counts its bytes like any other
+            if (elect_one()) {
+              mbar_arrive_expect_tx(full(s), L::ACT_BYTES);
+              tma_load_3d(dst, &act_map, full(s), 0, row0, u * L::BS);
+            }
           } else {
-            // the last unit's blocks
-            for (int b = 0; u * L::BS + b < kblocks; ++b)
-              mma_f16_ts_block(d_tmem, a_tmem + b * T_COLS, b_desc + ((b * L::BOX_BYTES) >> 4),
-                               idesc, b == 0 ? accumulate : 1u);
-            if (elect_one()) tc_commit(empty(s));
+            const int nb = min(L::BS, kblocks - u * L::BS);
+            if (elect_one()) mbar_arrive_expect_tx(full(s), nb * quads * 512);
+            __syncwarp();
+            for (int b = 0; b < nb; ++b)
+  #pragma unroll
+              for (int q = 0; q < PER_LANE; ++q)
+                if (lane + 32 * q < quads)
+                  tma_gather4(dst + b * L::BOX_BYTES + (lane + 32 * q) * 512, &act_map, full(s),
+                              (u * L::BS + b) * BK, src[q][0], src[q][1], src[q][2], src[q][3]);
           }
-          accumulate = 1;
+          ++it;
           if (++s == static_cast<uint32_t>(STAGES)) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (!ok) break;
-        if (elect_one()) tc_commit(dfull(acc));
-        if (u == u1) break;
       }
-      if (ACC == 2) acc ^= 1;
+      if (!ok && lane == 0) {  // let every copy already issued land
+        for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+          mbar_wait(full(i % STAGES), (i / STAGES) & 1u, never, nullptr, 100000000ull);
+      }
+    } else if (warp == 2) {
+      // ----------------------------------------------------- weight producer
+      uint32_t s = 0, ph = 0, issued = 0;
+      bool ok = true;
+      Item w;
+      for (int j = 0; ok && __any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w)); ++j) {
+        const size_t col = uniform(static_cast<uint32_t>(w.e * num_n + w.nt));  // 128-column run
+        const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));
+        const int kb0 = u0 * L::BS;
+        const uint8_t* wsrc = a.tiles + (col * kblocks + kb0) * WBLOCK_BYTES;
+        const __half* ssrc = a.scales + (col * groups + kb0 * BK / GROUP) * TILE_N;
+        for (int u = u0; u < u1; ++u) {
+          ok = mbar_wait_warp(wempty(s), ph ^ 1u, abort_flag, a.status, a.wait_limit_ns);
+          if (!ok) break;
+          // a whole unit's sizes are constants; one that starts inside a group
+          // of 128 (one block a unit) still needs that group
+          constexpr uint32_t kGroupsFull = (L::BS * BK + GROUP - 1) / GROUP;
+          uint32_t wbytes = L::BS * WBLOCK_BYTES, sbytes = kGroupsFull * TILE_N * 2;
+          if (L::BS > 1 && u == kunits - 1) {
+            const uint32_t nb = kblocks - u * L::BS;
+            wbytes = nb * WBLOCK_BYTES;
+            sbytes = (nb * BK + GROUP - 1) / GROUP * TILE_N * 2;
+          }
+          if (elect_one()) {
+            const uint32_t dst = w_base + s * L::W_SLOT;
+            mbar_arrive_expect_tx(wfull(s), wbytes + sbytes);
+            bulk_load(dst, wsrc, wbytes, wfull(s));
+            bulk_load(dst + L::BS * WBLOCK_BYTES, ssrc, sbytes, wfull(s));
+          }
+          wsrc += L::BS * WBLOCK_BYTES;
+          if (L::BS * BK >= GROUP || (u & 1)) ssrc += kGroupsFull * TILE_N;
+          ++issued;
+          if (++s == static_cast<uint32_t>(W_STAGES)) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (!ok && lane == 0) {  // let every copy already issued land
+        for (uint32_t i = issued > W_STAGES ? issued - W_STAGES : 0; i < issued; ++i)
+          mbar_wait(wfull(i % W_STAGES), (i / W_STAGES) & 1u, never, nullptr, 100000000ull);
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------- MMA issue
+      // Every loop bound is warp-uniform (see elect_one, uniform). The MMAs of a
+      // tall tile are as wide as its rows (rounded up to 16); below 64 rows the
+      // width costs no time and finding the rows would.
+      const uint64_t b_desc0 = smem_desc_sw128(act_base);
+      uint32_t s = 0, ph = 0;
+      uint32_t used[2] = {0, 0};  // segments committed per accumulator
+      int acc = 0;
+      bool ok = true;
+      Item w;
+      for (int j = 0; ok; ++j) {
+        uint32_t idesc = idesc_f16_f32(TILE_N, TILE_M);
+        if constexpr (TILE_M > 64) {
+          if (!__any_sync(0xffffffffu, item_at<TILE_M>(walk, j, w))) break;
+          idesc = idesc_f16_f32(TILE_N, static_cast<int>(uniform((w.rows + 15) & ~15)));
+        } else {
+          if (!__any_sync(0xffffffffu, span_at(walk, j, w.u0, w.u1))) break;
+        }
+        const int u1 = static_cast<int>(uniform(w.u1));
+        int u = static_cast<int>(uniform(w.u0));
+        const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
+        uint32_t accumulate = 0;  // the item's first MMA starts the sum
+        while (true) {
+          // one segment of at most kPromoteBlocks blocks, once the accumulator
+          // is free: the last item drained it, or the epilogue promoted it
+          const uint32_t n = acc == 0 ? used[0]++ : used[1]++;
+          ok = mbar_wait_warp(dempty(acc), (n & 1u) ^ 1u, abort_flag, a.status, a.wait_limit_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const int end = min(u1, u + kPromoteBlocks / L::BS);
+          for (; u < end; ++u) {
+            ok = mbar_wait_warp(full(s), ph, abort_flag, a.status, a.wait_limit_ns);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t b_desc = b_desc0 + ((s * L::ACT_BYTES) >> 4);
+            const uint32_t a_tmem = tmem_base + s * L::T_STAGE;
+            if (u * L::BS + L::BS <= kblocks) {
+              if constexpr (L::BS == 4)
+                mma_f16_ts_blocks4(d_tmem, a_tmem, b_desc, idesc, accumulate, L::BOX_BYTES >> 4,
+                                   empty(s));
+              else if constexpr (L::BS == 2)
+                mma_f16_ts_blocks2(d_tmem, a_tmem, b_desc, idesc, accumulate, L::BOX_BYTES >> 4,
+                                   empty(s));
+              else
+                mma_f16_ts_blocks1(d_tmem, a_tmem, b_desc, idesc, accumulate, empty(s));
+            } else {
+              // the last unit's blocks
+              for (int b = 0; u * L::BS + b < kblocks; ++b)
+                mma_f16_ts_block(d_tmem, a_tmem + b * T_COLS, b_desc + ((b * L::BOX_BYTES) >> 4),
+                                 idesc, b == 0 ? accumulate : 1u);
+              if (elect_one()) tc_commit(empty(s));
+            }
+            accumulate = 1;
+            if (++s == static_cast<uint32_t>(STAGES)) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+          if (!ok) break;
+          if (elect_one()) tc_commit(dfull(acc));
+          if (u == u1) break;
+        }
+        if (ACC == 2) acc ^= 1;
+      }
+      if (elect_one()) tc_commit(drain_bar);  // TMEM is freed only after every MMA completed
+      mbar_wait_warp(drain_bar, 0, never, nullptr, 100000000ull);
     }
-    if (elect_one()) tc_commit(drain_bar);  // TMEM is freed only after every MMA completed
-    mbar_wait_warp(drain_bar, 0, never, nullptr, 100000000ull);
   } else if (warp < L::FIRST_EPI_WARP) {
     // ---------------------------------------------------------------- dequant
-    const uint32_t dgroup = static_cast<uint32_t>(warp - FIRST_DEQ_WARP) >> 2;
+    if constexpr (L::SPLIT_REGS) regs_dec<64>();
+    const uint32_t dgroup = static_cast<uint32_t>(warp - L::FIRST_DEQ_WARP) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // weight column inside the tile
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
@@ -667,6 +678,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
     }
   } else {
     // --------------------------------------------------------------- epilogue
+    if constexpr (L::SPLIT_REGS) regs_inc<80>();
     constexpr int COLS = L::COLS;
     constexpr int EPI_THREADS = L::EPI_WARPS * 32;
     const int part = (warp - L::FIRST_EPI_WARP) >> 2;  // which accumulator columns

@@ -271,6 +271,18 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+// Registers a thread, from here on, of the four warps of an aligned warpgroup
+// (all of them execute it). What `regs_inc` takes has to come from what the
+// block was launched with and others gave back.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Warms L2 with a contiguous global range (16-byte aligned, size % 16 == 0).
 // Nothing lands in shared memory, so the range may still be written by an
 // earlier kernel: L2 is the point of coherence and later loads see the writes.
