@@ -342,10 +342,6 @@ int check_epilogue(const i4g_epilogue_t& e, int N) {
   return I4G_OK;
 }
 
-// Rows per weight that choose the tile height of an experts' product: the
-// mean over the experts that can have any.
-int mean_rows(int pairs, int E) { return (pairs + (pairs < E ? pairs : E) - 1) / (pairs < E ? pairs : E); }
-
 // Where a workspace holds the activations copied into row order (behind the
 // split tail's `split_bytes`, and behind the counters in any case), and the
 // workspace's size with them.
@@ -389,14 +385,14 @@ int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scal
                                             g_wait_limit_ns, static_cast<cudaStream_t>(stream)),
                   "decode kernel launch");
   }
-  const int tile_m = i4g::epi::choose_tile(offsets ? mean_rows(M, E) : M);
+  const int tile_m = i4g::epi::choose_tile(M, E, N, K, dev->sm_count);
   const long tiles_most = i4g::epi::tiles_bound(tile_m, M, E, N);
   // the workspace holds the split tail's part, then the activations in row
   // order where they are copied; each is used if it fits
   const size_t need = i4g::epi::workspace_bytes(tile_m, tiles_most, K, dev->sm_count);
   const bool split = workspace && need > 0 && workspace_bytes >= need;
-  if (rows && tile_m >= i4g::epi::kCopyRowsTile && workspace &&
-      workspace_bytes >= bytes_with_rows(need, M, K)) {
+  if (rows && workspace && workspace_bytes >= bytes_with_rows(need, M, K) &&
+      i4g::epi::copy_rows_first(tile_m, M, E, N, K, dev->sm_count)) {
     __half* copy = reinterpret_cast<__half*>(static_cast<char*>(workspace) + rows_offset(need));
     const cudaError_t g = i4g::epi::gather_rows(static_cast<const __half*>(A), a_rows, offsets,
                                                 rows, row_div, copy, M, E, K, dev->sm_count,
@@ -788,7 +784,7 @@ int i4g_gemm_epilogue_workspace_size(int M, int N, int K, size_t* bytes) {
   DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != I4G_OK) return st;
   if (i4g::epi::decode_is_faster(M, N, K, dev->sm_count)) return I4G_OK;  // needs none
-  const int tile_m = i4g::epi::choose_tile(M);
+  const int tile_m = i4g::epi::choose_tile(M, 1, N, K, dev->sm_count);
   *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, M, 1, N), K,
                                      dev->sm_count);
   return I4G_OK;
@@ -813,10 +809,11 @@ int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes) {
   if (pairs == 0) return I4G_OK;
   DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != I4G_OK) return st;
-  const int tile_m = i4g::epi::choose_tile(mean_rows(pairs, E));
+  const int tile_m = i4g::epi::choose_tile(pairs, E, N, K, dev->sm_count);
   *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, pairs, E, N), K,
                                      dev->sm_count);
-  if (tile_m >= i4g::epi::kCopyRowsTile) *bytes = bytes_with_rows(*bytes, pairs, K);
+  if (i4g::epi::copy_rows_first(tile_m, pairs, E, N, K, dev->sm_count))
+    *bytes = bytes_with_rows(*bytes, pairs, K);
   return I4G_OK;
 }
 

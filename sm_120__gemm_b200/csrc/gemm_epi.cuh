@@ -18,8 +18,9 @@
 //   known on the device, so each CTA first sums the experts' tile counts into
 //   a table in shared memory and everything else (which tile, which split)
 //   follows from that by arithmetic: no extra launch, nothing read back.
-// * Gathered activations come straight from the tokens' rows, four rows per
-//   TMA gather, so no permuted copy of A is written.
+// * Gathered activations of few rows come straight from the tokens' rows, four
+//   rows per TMA gather; where the gathers would cost more than a copy, they are
+//   copied into row order first (copy_rows_first).
 // * Small tiles (16, 32, 64 rows) for few rows per weight. There the weights
 //   bound it: 4 KB of codes per 64-k block and SM at HBM rate is a block every
 //   ~95 ns, and one dequant warp per SMSP needs several times that, so three
@@ -33,6 +34,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace i4g {
 namespace epi {
@@ -748,11 +750,16 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
         // ------------------------------------------------ whole tile -> C
         if (!ok) continue;
         tc_fence_after();
-        if (a.fp32_out) {
-#pragma unroll
-          for (int c = 0; c < COLS / 16; ++c) {
+        if constexpr (TILE_M == 128) {
+          // One chunk's code for all of them, up to the tile's last row: 64
+          // experts of 2048 x 4096 gated with 44 rows each 120 us unrolled,
+          // 94 so (at 16 to 64 rows a tile it is no faster).
+#pragma unroll 1
+          for (int c = 0; c < COLS / 16 && m0 + c * 16 < w.rows; ++c) {
             uint32_t v[16];
-            load_sum16(col0 + c * 16, &hb[c * 4], v);
+            load_sum16(col0 + c * 16, &hb[0], v);
+            rotate_down2(hb);
+            rotate_down2(hb);
             float f[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
@@ -762,36 +769,66 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(release_bar);
-        } else {
-          // rounded to FP16 pairs in registers, the accumulator released,
-          // then stored
-          constexpr int KEEP = GATED ? 8 : 16;  // values of a chunk this thread keeps
-          __half2 hv[COLS / 16 * KEEP / 2];
+          continue;
+        }
+        auto finish = [&](auto chunks) {
+          constexpr int CH = decltype(chunks)::value;  // 16-row chunks
+          if (a.fp32_out) {
 #pragma unroll
-          for (int c = 0; c < COLS / 16; ++c) {
-            uint32_t v[16];
-            load_sum16(col0 + c * 16, &hb[c * 4], v);
-            float f[16];
+            for (int c = 0; c < CH; ++c) {
+              uint32_t v[16];
+              load_sum16(col0 + c * 16, &hb[c * 4], v);
+              float f[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-            finish16<GATED>(sink, m0 + c * 16, up, f);
+              for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+              finish16<GATED>(sink, m0 + c * 16, up, f);
+              store16<GATED>(sink, m0 + c * 16, up, f);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(release_bar);
+          } else {
+            // rounded to FP16 pairs in registers, the accumulator released,
+            // then stored
+            constexpr int KEEP = GATED ? 8 : 16;  // values of a chunk this thread keeps
+            __half2 hv[CH * KEEP / 2];
 #pragma unroll
-            for (int i = 0; i < KEEP / 2; ++i)
-              hv[c * (KEEP / 2) + i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            for (int c = 0; c < CH; ++c) {
+              uint32_t v[16];
+              load_sum16(col0 + c * 16, &hb[c * 4], v);
+              float f[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+              finish16<GATED>(sink, m0 + c * 16, up, f);
+#pragma unroll
+              for (int i = 0; i < KEEP / 2; ++i)
+                hv[c * (KEEP / 2) + i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(release_bar);
+            __half* const cp = static_cast<__half*>(a.C) + sink.c0;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+              for (int i = 0; i < KEEP; ++i) {
+                const int m = m0 + c * 16 + i + (up ? 8 : 0);
+                const __half2 h = hv[c * (KEEP / 2) + i / 2];
+                if (m < w.rows)
+                  cp[static_cast<size_t>(m) * sink.ldc] = (i & 1) ? __high2half(h) : __low2half(h);
+              }
           }
+        };
+        // Tall tiles leave out rows past their last, by halves of a thread's
+        // columns (90 rows each: 164 us without, 157 so).
+        if (TILE_M < 256 || w.rows > m0 + COLS / 2) {
+          finish(std::integral_constant<int, COLS / 16>{});
+        } else if (w.rows > m0) {
+          if constexpr (TILE_M == 256) finish(std::integral_constant<int, COLS / 32>{});
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(release_bar);
-          __half* const cp = static_cast<__half*>(a.C) + sink.c0;
-#pragma unroll
-          for (int c = 0; c < COLS / 16; ++c)
-#pragma unroll
-            for (int i = 0; i < KEEP; ++i) {
-              const int m = m0 + c * 16 + i + (up ? 8 : 0);
-              const __half2 h = hv[c * (KEEP / 2) + i / 2];
-              if (m < w.rows)
-                cp[static_cast<size_t>(m) * sink.ldc] = (i & 1) ? __high2half(h) : __low2half(h);
-            }
         }
         continue;
       }

@@ -36,14 +36,15 @@ struct Sched {
   int full_tiles, tail_tiles, chunks;
 };
 
-// Activation rows per tile for `rows` rows per weight (16, 32, 64, 128, 256).
-int choose_tile(int rows);
+// Activation rows per tile (16, 32, 64, 128, 256) for M rows, of one weight or
+// spread over E experts.
+int choose_tile(int M, int E, int N, int K, int sm_count);
 // Whether the decode kernel's cluster schedule serves a dense product faster.
 bool decode_is_faster(int M, int N, int K, int sm_count);
-// Rows of a tile from which gathered activations are first copied into row
-// order by a kernel of their own (gather_rows) instead of four rows per copy
-// instruction inside the product.
-constexpr int kCopyRowsTile = 64;
+// Whether gathered activations are first copied into row order by a kernel of
+// their own (gather_rows) instead of four rows per copy instruction inside the
+// product.
+bool copy_rows_first(int tile_m, int M, int E, int N, int K, int sm_count);
 // 64-k blocks of the activation box of a tile height.
 int box_blocks(int tile_m);
 // out[p] = A[rows[p] / row_div] for p < offsets[E]; K halves a row.
