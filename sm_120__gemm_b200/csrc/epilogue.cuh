@@ -31,25 +31,38 @@ struct EpilogueOut {
   Epilogue epilogue;
 };
 
+// The hardware's 2^x and 1/x: within a few FP32 units in the last place, far
+// below the rounding to FP16; subnormals count as zeros.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.44269504f;
+
 // x * sigmoid(x (c0 + c1 x^2)): SiLU is c0 = 1, c1 = 0; tanh-GELU, whose
 // 0.5 (1 + tanh(u / 2)) is sigmoid(u), is c0 = sqrt(8/pi), c1 = 0.044715 c0.
-// 1 + exp(-u) overflows to infinity for very negative u and the quotient is
-// then the limit, -0. The fast exp and divide are each within a few FP32
-// units in the last place here, far below the rounding to FP16.
+// 1 + exp(-u) overflows to infinity for very negative u and the product is then
+// the limit, -0.
 __device__ __forceinline__ float sigmoid_gate(float x, float c0, float c1) {
   const float u = x * fmaf(c1 * x, x, c0);
-  return __fdividef(x, 1.0f + __expf(-u));
+  return x * rcp_fast(1.0f + exp2_fast(-kLog2e * u));
 }
 
 // GELU x Phi(x) = max(x, 0) - |x| erfc(z) / 2 with z = |x| / sqrt 2: no
 // cancellation on the negative side. erfc(z) exp(z^2) is a polynomial of degree
 // 8 in t = 1 / (1 + z / 2), times t, fitted by weighted least squares for the
 // least largest relative error (4e-8; 3.3e-7 evaluated in FP32): 20
-// instructions (M = 203, N = 14336, whose one wave of tiles hides no epilogue:
-// 36.2 us, and 41.6 with the library's erfc).
+// instructions, 5.4 us less than the library's erfc in a product of M = 203,
+// K = 4096, N = 14336, whose one wave of tiles hides no epilogue.
 __device__ __forceinline__ float gelu_erf(float x) {
   const float a = fminf(fabsf(x), 40.0f);  // exp(-800) is 0: infinities keep their limits
-  const float t = __fdividef(1.0f, fmaf(a, 0.35355339f, 1.0f));
+  const float t = rcp_fast(fmaf(a, 0.35355339f, 1.0f));
   float p = -0.05889091f;
   p = fmaf(p, t, 0.28370258f);
   p = fmaf(p, t, -0.48538491f);
@@ -59,7 +72,7 @@ __device__ __forceinline__ float gelu_erf(float x) {
   p = fmaf(p, t, 0.24326095f);
   p = fmaf(p, t, 0.28235349f);
   p = fmaf(p, t, 0.28208768f);
-  const float h = 0.5f * a * (p * t) * __expf(-0.5f * a * a);
+  const float h = 0.5f * a * (p * t) * exp2_fast((-0.5f * kLog2e) * a * a);
   return x < 0.0f ? -h : x - h;
 }
 

@@ -34,7 +34,6 @@
 
 #include <algorithm>
 #include <climits>
-#include <type_traits>
 
 namespace i4g {
 namespace epi {
@@ -750,32 +749,12 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
         // ------------------------------------------------ whole tile -> C
         if (!ok) continue;
         tc_fence_after();
-        if constexpr (TILE_M == 128) {
-          // One chunk's code for all of them, up to the tile's last row: 64
-          // experts of 2048 x 4096 gated with 44 rows each 120 us unrolled,
-          // 94 so (at 16 to 64 rows a tile it is no faster).
-#pragma unroll 1
-          for (int c = 0; c < COLS / 16 && m0 + c * 16 < w.rows; ++c) {
-            uint32_t v[16];
-            load_sum16(col0 + c * 16, &hb[0], v);
-            rotate_down2(hb);
-            rotate_down2(hb);
-            float f[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-            finish16<GATED>(sink, m0 + c * 16, up, f);
-            store16<GATED>(sink, m0 + c * 16, up, f);
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(release_bar);
-          continue;
-        }
-        auto finish = [&](auto chunks) {
-          constexpr int CH = decltype(chunks)::value;  // 16-row chunks
+        if constexpr (TILE_M <= 64) {
+          // Small tiles run this tens of times a CTA: unrolled, and a chunk's
+          // rows are not looked at (7 rows each 64 us so, 66 rolled).
           if (a.fp32_out) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
+            for (int c = 0; c < COLS / 16; ++c) {
               uint32_t v[16];
               load_sum16(col0 + c * 16, &hb[c * 4], v);
               float f[16];
@@ -791,9 +770,9 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
             // rounded to FP16 pairs in registers, the accumulator released,
             // then stored
             constexpr int KEEP = GATED ? 8 : 16;  // values of a chunk this thread keeps
-            __half2 hv[CH * KEEP / 2];
+            __half2 hv[COLS / 16 * KEEP / 2];
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
+            for (int c = 0; c < COLS / 16; ++c) {
               uint32_t v[16];
               load_sum16(col0 + c * 16, &hb[c * 4], v);
               float f[16];
@@ -809,7 +788,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
             if (lane == 0) mbar_arrive(release_bar);
             __half* const cp = static_cast<__half*>(a.C) + sink.c0;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+            for (int c = 0; c < COLS / 16; ++c)
 #pragma unroll
               for (int i = 0; i < KEEP; ++i) {
                 const int m = m0 + c * 16 + i + (up ? 8 : 0);
@@ -818,17 +797,74 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
                   cp[static_cast<size_t>(m) * sink.ldc] = (i & 1) ? __high2half(h) : __low2half(h);
               }
           }
-        };
-        // Tall tiles leave out rows past their last, by halves of a thread's
-        // columns (90 rows each: 164 us without, 157 so).
-        if (TILE_M < 256 || w.rows > m0 + COLS / 2) {
-          finish(std::integral_constant<int, COLS / 16>{});
-        } else if (w.rows > m0) {
-          if constexpr (TILE_M == 256) finish(std::integral_constant<int, COLS / 32>{});
-        } else {
+          continue;
+        }
+        // In tall tiles the loops over 16-row chunks stay rolled and end at
+        // the tile's last row: a CTA runs them a few times, and fetching
+        // unrolled code costs more than the branches (M = 203, K = 4096,
+        // N = 14336 with GELU 36.5 us unrolled, 32.6 so; 64 experts of
+        // 2048 x 4096 with 44 rows each, 128-row tiles, 120 / 94).
+        if (TILE_M == 128 || a.fp32_out) {
+#pragma unroll 1
+          for (int c = 0; c < COLS / 16; ++c) {
+            if (m0 + c * 16 >= w.rows) break;
+            uint32_t v[16];
+            load_sum16(col0 + c * 16, &hb[0], v);
+            rotate_down2(hb);
+            rotate_down2(hb);
+            float f[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+            finish16<GATED>(sink, m0 + c * 16, up, f);
+            store16<GATED>(sink, m0 + c * 16, up, f);
+          }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(release_bar);
+        } else {
+          // Values are rounded to FP16 pairs in registers, the accumulator
+          // released (at 256 rows the MMAs wait for it), then stored. The pairs
+          // move down a chunk a step, so that register indices are fixed.
+          constexpr int PAIRS = GATED ? 4 : 8;  // of a chunk that this thread keeps
+          constexpr int KEPT = COLS / 16 * PAIRS;
+          __half2 hv[KEPT];
+#pragma unroll
+          for (int q = 0; q < KEPT; ++q) hv[q] = __half2();
+#pragma unroll 1
+          for (int c = 0; c < COLS / 16; ++c) {
+#pragma unroll
+            for (int q = 0; q + PAIRS < KEPT; ++q) hv[q] = hv[q + PAIRS];
+            if (m0 + c * 16 < w.rows) {
+              uint32_t v[16];
+              load_sum16(col0 + c * 16, &hb[0], v);
+              rotate_down2(hb);
+              rotate_down2(hb);
+              float f[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+              finish16<GATED>(sink, m0 + c * 16, up, f);
+#pragma unroll
+              for (int i = 0; i < PAIRS; ++i)
+                hv[KEPT - PAIRS + i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(release_bar);
+          __half* const cp = static_cast<__half*>(a.C) + sink.c0;
+#pragma unroll 1
+          for (int c = 0; c < COLS / 16; ++c) {
+            if (m0 + c * 16 >= w.rows) break;
+#pragma unroll
+            for (int i = 0; i < 2 * PAIRS; ++i) {
+              const int m = m0 + c * 16 + i + (up ? 8 : 0);
+              if (m < w.rows)
+                cp[static_cast<size_t>(m) * sink.ldc] =
+                    (i & 1) ? __high2half(hv[i / 2]) : __low2half(hv[i / 2]);
+            }
+#pragma unroll
+            for (int q = 0; q + PAIRS < KEPT; ++q) hv[q] = hv[q + PAIRS];
+          }
         }
         continue;
       }
