@@ -83,8 +83,8 @@ int choose_tile(int M, int E, int N, int K, int sm_count) {
   };
   static constexpr Line kLines[] = {
       {16, 4.5, 0.106, 0.0, 4.4, 0.8},     {32, 5.7, 0.114, 0.0, 6.2, 1.7},
-      {64, 5.7, 0.128, 0.0, 8.6, 1.9},     {128, 4.7, 0.120, 0.088, 13.5, 2.2},
-      {256, 5.0, 0.179, 0.203, 15.2, 4.0},
+      {64, 5.7, 0.128, 0.0, 8.6, 1.9},     {128, 6.0, 0.120, 0.088, 13.5, 2.2},
+      {256, 6.5, 0.179, 0.203, 15.2, 4.0},
   };
   int best = 256;
   double least = 0.0;

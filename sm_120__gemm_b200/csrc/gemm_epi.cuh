@@ -8,7 +8,7 @@
 // Mathematics and accuracy are those of gemm_tc.cu: swap-AB (MMA-M = 128
 // weight columns from TMEM, MMA-N = TILE_M activation rows from 128B-swizzled
 // shared memory), weights dequantised to the exact half(q * s), FP32
-// accumulation with a promotion every kPromoteBlocks blocks. Different here:
+// accumulation with a promotion every promote_blocks. Different here:
 //
 // * The epilogue (epilogue.cuh) runs on the FP32 sums in registers. A thread
 //   holds one weight column; of a gated pair the two columns sit 8 lanes
@@ -48,7 +48,12 @@ constexpr int BK = 64;
 constexpr int T_COLS = 32;                     // TMEM columns per weight stage
 constexpr int TMEM_COLS = 512;
 constexpr int WBLOCK_BYTES = TILE_N * BK / 2;  // 4096
-constexpr int kPromoteBlocks = 32;             // 2048 k, as gemm_tc.cu
+// Blocks after which the accumulator is promoted: 2048 k, as gemm_tc.cu, where
+// the result is rounded to FP16; 512 k for FP32 results, which would show the
+// tensor core's drift. M = 300, N = 4096, K = 8192 in FP32, off by (2-norm,
+// relative): 2.5e-6 at 2048 k (31 us), 6.7e-7 at 512 k (43 us), 6.0e-7 a product
+// with FP32 multiply-adds.
+__host__ __device__ constexpr int promote_blocks(bool fp32_out) { return fp32_out ? 8 : 32; }
 constexpr int kTableInts = kMaxExperts + 1 + 32;
 
 template <int TILE_M>
@@ -326,6 +331,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
   const int kunits = (kblocks + L::BS - 1) / L::BS;
   const int groups = a.K / GROUP;
   const int num_n = a.N / TILE_N;
+  const int seg = promote_blocks(a.fp32_out) / L::BS;  // units between promotions
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -539,13 +545,13 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
         const uint32_t d_tmem = tmem_base + L::ACC_COL + acc * TILE_M;
         uint32_t accumulate = 0;  // the item's first MMA starts the sum
         while (true) {
-          // one segment of at most kPromoteBlocks blocks, once the accumulator
+          // one segment of at most promote_blocks, once the accumulator
           // is free: the last item drained it, or the epilogue promoted it
           const uint32_t n = acc == 0 ? used[0]++ : used[1]++;
           ok = mbar_wait_warp(dempty(acc), (n & 1u) ^ 1u, abort_flag, a.status, a.wait_limit_ns);
           if (!ok) break;
           tc_fence_after();
-          const int end = min(u1, u + kPromoteBlocks / L::BS);
+          const int end = min(u1, u + seg);
           for (; u < end; ++u) {
             ok = mbar_wait_warp(full(s), ph, abort_flag, a.status, a.wait_limit_ns);
             if (!ok) break;
@@ -713,8 +719,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
                       ? __half2float(a.epilogue.bias[static_cast<size_t>(w.e) * a.N +
                                                      w.nt * TILE_N + row])
                       : 0.0f;
-      constexpr int kSeg = kPromoteBlocks / L::BS;  // units per segment
-      const int nseg = (w.u1 - w.u0 + kSeg - 1) / kSeg;
+      const int nseg = (w.u1 - w.u0 + seg - 1) / seg;
       uint32_t hb[COLS / 4];  // the running sum's high parts (e5m2 x4)
 #pragma unroll
       for (int q = 0; q < COLS / 4; ++q) hb[q] = 0u;

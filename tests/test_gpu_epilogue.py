@@ -62,6 +62,18 @@ def test_groups_and_types(i4g, group, M, fp32):
     run(i4g, M, 256, 384, group, "gelu", gated=(group == 64), bias=True, residual=True, fp32=fp32)
 
 
+# every tile height in turn, by threes and fours: 32, 64, 128 and 256 rows (the
+# height follows from how many tiles the SMs get, so small shapes take 16)
+@pytest.mark.parametrize("M,N,K", [(17, 18944, 1088), (25, 20480, 2048), (90, 2432, 12416),
+                                   (33, 18944, 1088), (63, 14336, 2112), (160, 4096, 4160),
+                                   (65, 9600, 2112), (127, 18944, 1088), (513, 9472, 1088),
+                                   (1000, 1920, 4160), (129, 18944, 576), (203, 18944, 320),
+                                   (255, 18944, 576), (203, 9600, 8256)])
+@pytest.mark.parametrize("gated,fp32", [(False, False), (True, False), (False, True)])
+def test_tile_heights(i4g, M, N, K, gated, fp32):
+    run(i4g, M, N, K, 64, "gelu" if gated else "none", gated, bias=True, residual=True, fp32=fp32)
+
+
 # tails cut along K: few tiles and long K, more tiles than SMs, promotion; up to
 # 16 rows both kernels that serve them
 @pytest.mark.parametrize("M,N,K", [(1, 128, 14336), (7, 256, 8192), (1, 28672, 2048),

@@ -202,6 +202,18 @@ def test_experts_split_tails(i4g, T, E, k, K, N):
         assert torch.equal(ex(a, r, activation="silu", gated=True)[:n], first[:n])
 
 
+# tiles of 32 rows (the first two), 64, 128 and 256
+@pytest.mark.parametrize("T,E,k,K,N", [(100, 8, 2, 1088, 4864), (150, 4, 2, 4160, 1280),
+                                       (240, 8, 2, 1088, 4864), (350, 4, 2, 4160, 1280),
+                                       (450, 8, 2, 320, 4864), (1200, 5, 1, 576, 4864),
+                                       (1500, 5, 2, 576, 4864), (700, 3, 1, 4160, 4864)])
+@pytest.mark.parametrize("kind,gather", [("random", True), ("skewed", True), ("padded", False)])
+def test_experts_tile_heights(i4g, T, E, k, K, N, kind, gather):
+    if kind == "skewed" and k == 1:
+        kind = "one"  # a token has one expert: all of them the first
+    check_experts(i4g, kind, T, E, k, K, N, 64, "silu", True, True, gather)
+
+
 def test_experts_fp32_one_expert_and_many(i4g):
     check_experts(i4g, "one", 30, 1, 1, 128, 128, 32, fp32=True, bias=True)
     check_experts(i4g, "padded", 40, 512, 4, 64, 128, 64, "relu")
