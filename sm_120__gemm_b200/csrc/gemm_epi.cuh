@@ -49,11 +49,15 @@ constexpr int T_COLS = 32;                     // TMEM columns per weight stage
 constexpr int TMEM_COLS = 512;
 constexpr int WBLOCK_BYTES = TILE_N * BK / 2;  // 4096
 // Blocks after which the accumulator is promoted: 2048 k, as gemm_tc.cu, where
-// the result is rounded to FP16; 512 k for FP32 results, which would show the
-// tensor core's drift. M = 300, N = 4096, K = 8192 in FP32, off by (2-norm,
-// relative): 2.5e-6 at 2048 k (31 us), 6.7e-7 at 512 k (43 us), 6.0e-7 a product
-// with FP32 multiply-adds.
-__host__ __device__ constexpr int promote_blocks(bool fp32_out) { return fp32_out ? 8 : 32; }
+// the result is rounded to FP16; 512 k (256 in small tiles, where that costs a
+// few per cent) for FP32 results, which would show the tensor core's drift.
+// M = 300, N = 4096, K = 8192 in FP32, off by (2-norm, relative): 2.5e-6 at
+// 2048 k (31 us), 6.7e-7 at 512 k (43 us), 6.0e-7 a product with FP32
+// multiply-adds.
+template <int TILE_M>
+__host__ __device__ constexpr int promote_blocks(bool fp32_out) {
+  return fp32_out ? (TILE_M <= 64 ? 4 : 8) : 32;
+}
 constexpr int kTableInts = kMaxExperts + 1 + 32;
 
 template <int TILE_M>
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
   const int kunits = (kblocks + L::BS - 1) / L::BS;
   const int groups = a.K / GROUP;
   const int num_n = a.N / TILE_N;
-  const int seg = promote_blocks(a.fp32_out) / L::BS;  // units between promotions
+  const int seg = promote_blocks<TILE_M>(a.fp32_out) / L::BS;  // units between promotions
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
