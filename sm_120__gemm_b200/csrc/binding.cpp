@@ -1,7 +1,7 @@
 // Host path of the operators' Python entry points (linear.py, experts.py): the
 // checks of their tensors, their outputs and workspaces, and the call of the
 // C ABI. In Python the same work took 11-18 us a call, several times the
-// kernels of a single token (routing 18.2 -> 9.2 us, combination 10.5 -> 5.3 us).
+// kernels of a single token (routing 18.2 -> 7.3 us, combination 10.5 -> 5.5 us).
 //
 // Every function runs on the current device's current stream; the Python side
 // makes the tensors' device and the caller's stream current first.
@@ -66,6 +66,17 @@ const void* ptr(const OptTensor& t) { return t ? t->const_data_ptr() : nullptr; 
 
 Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, at::Device device) {
   return Tensor(at::detail::empty_cuda(shape, dtype, device, std::nullopt));
+}
+
+// Contiguous tensor of 32-bit values inside `whole`, from its next free value on
+// (`at`, moved past it to a multiple of 16 bytes).
+Tensor part(const Tensor& whole, at::IntArrayRef shape, at::ScalarType dtype, int64_t& at) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(dtype));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  at += (t.numel() + 3) / 4 * 4;
+  return t;
 }
 
 int narrow(int64_t v, const char* name) {
@@ -232,11 +243,14 @@ py::tuple route(const Tensor& logits_in, int64_t top_k, int64_t scoring, const O
   const int64_t pairs = T * k;
   size_t need = 0;
   check("i4g_route_workspace_size", i4g_route_workspace_size(t, experts, &need));
-  Tensor ids = empty({T, k}, at::kInt, on.device);
-  Tensor weights = empty({T, k}, at::kFloat, on.device);
-  Tensor offsets = empty({E + 1}, at::kInt, on.device);
-  Tensor rows = empty({pairs}, at::kInt, on.device);
-  Tensor slots = empty({T, k}, at::kInt, on.device);
+  // the five results in one allocation: one token's call 9.4 -> 7.3 us
+  int64_t at = 0;
+  const Tensor whole = empty({4 * ((pairs + 3) / 4 * 4) + (E + 4) / 4 * 4}, at::kInt, on.device);
+  Tensor ids = part(whole, {T, k}, at::kInt, at);
+  Tensor weights = part(whole, {T, k}, at::kFloat, at);
+  Tensor offsets = part(whole, {E + 1}, at::kInt, at);
+  Tensor rows = part(whole, {pairs}, at::kInt, at);
+  Tensor slots = part(whole, {T, k}, at::kInt, at);
   Tensor ws;  // for the counts; nothing is kept in it
   if (need) ws = empty({static_cast<int64_t>(need)}, at::kByte, on.device);
   i4g_route_t o{static_cast<int>(scoring),     narrow(n_group, "n_group"),

@@ -24,7 +24,8 @@ from .linear import interleave_gate_up
 
 
 class Routing(NamedTuple):
-    """A batch's routing. A pair is token * top_k + place."""
+    """A batch's routing (from `route`: five tensors in one allocation). A pair is
+    token * top_k + place."""
     ids: torch.Tensor      # int32 [T, top_k]: experts, best first (-1: none)
     weights: torch.Tensor  # float32 [T, top_k]
     offsets: torch.Tensor  # int32 [E + 1]: expert e has sorted rows offsets[e] .. offsets[e + 1]

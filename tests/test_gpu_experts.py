@@ -129,6 +129,18 @@ def test_route_strided_empty_and_streams(i4g):
         i4g.route(wide.double(), 4)
 
 
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (5, 7, 3), (40, 65, 5)])
+def test_route_results_do_not_overlap(i4g, T, E, k):
+    x = rand(T, E, seed=3, dtype=torch.float32)
+    want = [t.clone() for t in i4g.route(x, k)]
+    for i in range(5):
+        got = i4g.route(x, k)
+        assert all(t.is_contiguous() and t.data_ptr() % 16 == 0 for t in got)
+        got[i].fill_(-7)
+        assert (got[i] == -7).all()
+        assert all(torch.equal(a, b) for j, (a, b) in enumerate(zip(got, want)) if j != i)
+
+
 def routing_of(i4g, ids, E):
     offsets, rows, slots = ref.order(ids, E)
     T, k = ids.shape
