@@ -214,7 +214,7 @@ int main() {
 
 
 def test_plain_routing_of_a_worked_example():
-    """The checker itself, on numbers worked by hand."""
+    """The comparison itself, on numbers worked by hand."""
     import operators_ref as ref
     x = torch.tensor([[0.0, 2.0, 2.0, 1.0], [-np.inf] * 4, [np.nan, 1.0, -np.inf, 3.0]])
     ids, w, off, rows, slots = ref.route(x, 2)
@@ -231,7 +231,7 @@ def test_plain_routing_of_a_worked_example():
 
 
 def test_routings_agree():
-    """The checker and the definition that the timed cases use pick the same."""
+    """The plain routing and the definition that the timed cases use pick the same."""
     import importlib.util
     import os
 
