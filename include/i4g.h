@@ -286,9 +286,11 @@ int i4g_route(const void* logits, int fp32_logits, int ld_logits, const float* b
  * offsets[E] are left as they were. The epilogue has no residual (it belongs
  * to i4g_experts_combine). offsets and rows are read on the device; offsets
  * outside [0, pairs] are clamped, rows outside A read as zeros. E <= 512.
- * workspace: as for i4g_gemm_epilogue; for many gathered rows per expert it
- * also holds them in expert order (its counters are the first 4096 bytes
- * either way). pairs = 0 returns at once. */
+ * workspace: as for i4g_gemm_epilogue; where gathered rows are worth a copy
+ * into expert order it also holds that copy (its counters are the first 4096
+ * bytes either way). The size is for these arguments, and fewer pairs can ask
+ * for more; a call with less than it asks for is slower, not wrong. pairs = 0
+ * returns at once. */
 int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes);
 int i4g_experts_gemm(const void* A, int a_rows, const uint8_t* tiles, const void* scales, void* C,
                      const int32_t* offsets, const int32_t* rows, int row_div, int pairs, int E,

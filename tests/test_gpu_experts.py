@@ -226,6 +226,31 @@ def test_experts_tile_heights(i4g, T, E, k, K, N, kind, gather):
     check_experts(i4g, kind, T, E, k, K, N, 64, "silu", True, True, gather)
 
 
+# without a workspace nothing is split or copied ahead: tokens' rows are gathered
+# inside the product at every tile height
+@pytest.mark.parametrize("T,E,k,K,N", [(9, 8, 2, 320, 384), (100, 8, 2, 1088, 4864),
+                                       (240, 8, 2, 1088, 4864), (450, 8, 2, 320, 4864),
+                                       (1500, 5, 2, 576, 4864)])
+@pytest.mark.parametrize("kind", ["random", "padded"])
+def test_experts_without_a_workspace(i4g, T, E, k, K, N, kind):
+    w = rand(E, K, N, seed=1, scale=0.05)
+    ex = i4g.QuantizedExperts.from_weight(w, 64)
+    r = routing_of(i4g, choices(kind, T, E, k), E)
+    a = rand(T, K, seed=2)
+    got = torch.full((T * k, N), 77.0, dtype=torch.float16, device="cuda")
+    i4g.launch_experts(a, T, ex.tiles, ex.scales, got, r.offsets, r.rows, k, T * k, E, N, K, 64,
+                       activation="relu")
+    torch.cuda.synchronize()
+    assert i4g.device_status() == 0
+    edges = r.offsets.tolist()
+    for e in range(E):
+        lo, hi = edges[e], edges[e + 1]
+        if lo < hi:
+            src = a[(r.rows[lo:hi] // k).long()]
+            ref.check(got[lo:hi], *ref.linear(src, ref.weight(w[e], 64), "relu"))
+    assert (got[edges[E]:] == 77).all()
+
+
 def test_experts_fp32_one_expert_and_many(i4g):
     check_experts(i4g, "one", 30, 1, 1, 128, 128, 32, fp32=True, bias=True)
     check_experts(i4g, "padded", 40, 512, 4, 64, 128, 64, "relu")
