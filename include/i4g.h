@@ -285,7 +285,8 @@ int i4g_route(const void* logits, int fp32_logits, int ld_logits, const float* b
  * one after another. C and the sorted rows have `pairs` rows; those past
  * offsets[E] are left as they were. The epilogue has no residual (it belongs
  * to i4g_experts_combine). offsets and rows are read on the device; offsets
- * outside [0, pairs] are clamped, rows outside A read as zeros. E <= 512.
+ * outside [0, pairs] are clamped, and where one is then below the one before
+ * it no row of C is written; rows outside A read as zeros. E <= 512.
  * workspace: as for i4g_gemm_epilogue; where gathered rows are worth a copy
  * into expert order it also holds that copy (its counters are the first 4096
  * bytes either way). The size is for these arguments, and fewer pairs can ask

@@ -400,12 +400,17 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
   grid_dependency_wait();
   if (threadIdx.x == 0) launch_dependents();
   if (a.offsets) {
-    // m-tiles before each expert
+    // m-tiles before each expert. Offsets that fall would let rows belong to
+    // several experts, and so make more tiles than the grid and the workspace
+    // are for (16 experts, 64 rows, offsets 0 64 0 64 ...: 11 partial tiles
+    // behind the workspace's end); such a table has no tiles at all.
     const int e = threadIdx.x;
     int sum = 0;
+    bool falls = false;
     if (e < a.E) {
       const int lo = min(max(a.offsets[e], 0), a.M);
-      const int hi = min(max(a.offsets[e + 1], lo), a.M);
+      const int hi = min(max(a.offsets[e + 1], 0), a.M);
+      falls = hi < lo;
       sum = (hi - lo + TILE_M - 1) / TILE_M;
     }
 #pragma unroll
@@ -414,13 +419,13 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
       if (lane >= d) sum += o;
     }
     if (lane == 31) table[kMaxExperts + 1 + warp] = sum;
-    __syncthreads();
+    const bool ascending = !__syncthreads_or(falls);
     for (int i = 0; i < warp; ++i) sum += table[kMaxExperts + 1 + i];
     if (e < a.E) table[e + 1] = sum;
     if (e == 0) table[0] = 0;
     __syncthreads();
-    walk.s = make_sched(table[a.E] * num_n, kunits, L::BS, gridDim.x, a.tickets != nullptr,
-                        split_overhead_blocks<TILE_M>());
+    walk.s = make_sched(ascending ? table[a.E] * num_n : 0, kunits, L::BS, gridDim.x,
+                        a.tickets != nullptr, split_overhead_blocks<TILE_M>());
     walk.start();
   }
 

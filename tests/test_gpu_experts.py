@@ -297,6 +297,37 @@ def test_experts_bad_tables_are_clamped(i4g):
     assert i4g.device_status() == 0
 
 
+def test_experts_offsets_that_fall_stay_in_the_workspace(i4g):
+    """Offsets that fall and rise again name more tiles than any routing: nothing is
+    written, neither to C nor behind the workspace (guards of 1 MB around both)."""
+    E, K, N, M = 16, 8192, 128, 64
+    ex = i4g.QuantizedExperts.from_weight(rand(E, K, N, seed=1, scale=0.05), 64)
+    a = rand(M, K, seed=2)
+    need = i4g.experts_workspace_size(M, E, N, K)
+    assert need > 4096
+    guard = 1 << 20
+    held = torch.full((guard + need + guard,), 9, dtype=torch.uint8, device="cuda")
+    ws = held[guard:guard + need]
+    ws.zero_()
+    out = torch.full((M, N), 5.0, dtype=torch.float16, device="cuda")
+    rows = torch.arange(M, dtype=torch.int32, device="cuda")
+    for offsets in ([0, M] * 8 + [0], [0] + [M, 0] * 8, [0] * 15 + [M, M - 1]):
+        t = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+        for r in (None, rows):
+            i4g.launch_experts(a, M, ex.tiles, ex.scales, out, t, r, 1, M, E, N, K, 64,
+                               workspace=ws)
+    torch.cuda.synchronize()
+    assert i4g.device_status() == 0
+    assert (out == 5).all() and not ws[:4096].any()
+    assert (held[:guard] == 9).all() and (held[guard + need:] == 9).all()
+    # and the workspace still serves a routing
+    t = torch.arange(E + 1, dtype=torch.int32, device="cuda") * (M // E)
+    i4g.launch_experts(a, M, ex.tiles, ex.scales, out, t, None, 1, M, E, N, K, 64, workspace=ws)
+    other = torch.empty_like(out)
+    i4g.launch_experts(a, M, ex.tiles, ex.scales, other, t, None, 1, M, E, N, K, 64)
+    assert (out != 5).any() and (out - other).abs().max() <= 2.0 ** -9 * other.abs().max()
+
+
 @pytest.mark.parametrize("T,k,N", [(1, 1, 8), (1, 8, 4096), (7, 2, 1000), (300, 8, 256),
                                    (40, 32, 64), (65, 11, 136)])
 @pytest.mark.parametrize("residual", [False, True])
