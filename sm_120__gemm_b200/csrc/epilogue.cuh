@@ -47,10 +47,12 @@ constexpr float kLog2e = 1.44269504f;
 
 // x * sigmoid(x (c0 + c1 x^2)): SiLU is c0 = 1, c1 = 0; tanh-GELU, whose
 // 0.5 (1 + tanh(u / 2)) is sigmoid(u), is c0 = sqrt(8/pi), c1 = 0.044715 c0.
-// 1 + exp(-u) overflows to infinity for very negative u and the product is then
-// the limit, -0.
+// x^2 is capped so that c1 = 0 takes it out for infinite x too (0 times
+// infinity is a NaN); tanh-GELU's u is beyond every exponent there anyway.
+// +infinity gives +infinity; 1 + exp(-u) overflows to infinity for very
+// negative finite x and the product is then the limit, -0.
 __device__ __forceinline__ float sigmoid_gate(float x, float c0, float c1) {
-  const float u = x * fmaf(c1 * x, x, c0);
+  const float u = x * fmaf(c1, fminf(x * x, 1e30f), c0);
   return x * rcp_fast(1.0f + exp2_fast(-kLog2e * u));
 }
 

@@ -119,6 +119,27 @@ def test_large_values_saturate_like_fp16(i4g):
     assert (got[x < -1000] == 0).all()
 
 
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_infinity_stays_infinity(i4g, act, gated, M):
+    """act(+infinity) is +infinity for every activation: from a bias, and from a
+    sum of an infinite activation row; gated, it takes the sign of the up column."""
+    lin, w64 = make(i4g, 128, 256, 64)
+    a = rand(M, 128, seed=2)
+    bias = rand(256, seed=3)
+    bias[[2, 21, 199]] = float("inf")  # gate columns, were they gated
+    want, tol = ref.linear(a, w64, act, gated, bias)
+    got = lin(a, activation=act, gated=gated, bias=bias)
+    lost = torch.isinf(want)
+    assert int(lost.sum()) == 3 * M and torch.equal(got[lost].double(), want[lost])
+    ref.check(got[~lost], want[~lost], tol[~lost])
+    a = torch.zeros_like(a)
+    a[1, 7] = float("inf")
+    got = lin(a, activation=act)
+    assert torch.isposinf(got[1, w64[7] > 0]).all()
+
+
 def test_residual_in_place_strided_and_out(i4g):
     lin, w64 = make(i4g, 512, 256, 128)
     a = rand(33, 512, seed=7)
