@@ -127,6 +127,17 @@ __device__ __forceinline__ float weight_of(float x, float top, int sigmoid, floa
   if (sigmoid) return 1.0f / (1.0f + expf(-x));
   return (x == top ? 1.0f : expf(x - top)) / sum;
 }
+// The same in FP64, for scores near or below FP32's smallest normal number
+// (e^-87.3), where the FP32 form has lost bits or is 0: a token whose chosen
+// experts all lie there still has weights, divided by their sum.
+constexpr float kSmallScore = -80.0f;  // of the logit, or of its distance to the largest
+__device__ __forceinline__ bool small_score(float x, float top, int sigmoid) {
+  return (sigmoid ? x : x - top) < kSmallScore;
+}
+__device__ __forceinline__ double small_weight_of(float x, float top, int sigmoid, float sum) {
+  if (sigmoid) return 1.0 / (1.0 + exp(-static_cast<double>(x)));
+  return (x == top ? 1.0 : exp(static_cast<double>(x) - top)) / sum;
+}
 
 // Lane's experts by falling key, the lower index first among equal keys:
 // adjacent exchanges of strictly rising neighbours only, so ties keep their
@@ -327,10 +338,19 @@ __device__ __forceinline__ int route_token(const Args& a, int t, int lane,
     scores(x, top, a.sigmoid, pd);
     choose(a, lane, x, pd, bias, by_score, 0.0, id);
   }
-  float w = 0.0f;  // lane i: expert id's score
-  if (id >= 0)
-    w = weight_of(static_cast<float>(logits_of<FP32>(a, t)[id]), top, a.sigmoid, sum);
-  if (a.renormalize) {
+  float xi = 0.0f, w = 0.0f;  // lane i: expert id's logit and score
+  if (id >= 0) {
+    xi = static_cast<float>(logits_of<FP32>(a, t)[id]);
+    w = weight_of(xi, top, a.sigmoid, sum);
+  }
+  if (__any_sync(kAll, id >= 0 && small_score(xi, top, a.sigmoid))) {
+    double wd = id >= 0 ? small_weight_of(xi, top, a.sigmoid, sum) : 0.0;
+    if (a.renormalize) {
+      const double all = warp_sum(wd);
+      wd = all > 0.0 ? wd / all : 0.0;
+    }
+    w = static_cast<float>(wd);
+  } else if (a.renormalize) {
     const float all = warp_sum(w);
     w = all > 0.0f ? w / all : 0.0f;
   }

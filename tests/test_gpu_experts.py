@@ -97,6 +97,35 @@ def test_route_masks_infinities_and_nan(i4g):
     assert not (r.ids == 3).any() and not (r.ids == 9).any() and (r.ids[:, 30:] == -1).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("T", [12, 700])
+def test_route_weights_of_scores_below_fp32(i4g, dtype, T):
+    """Chosen experts whose scores FP32 cannot hold still share a token's weight:
+    FP64 holds sigmoids of logits down to -708 (and gives 0 for the last row's)."""
+    x = rand(T, 40, seed=T, scale=2.0, dtype=torch.float32)
+    top = torch.tensor([-60.0, -79.0, -81.0, -86.0, -87.3, -88.0, -89.0, -95.0, -120.0, -300.0,
+                        -650.0, -900.0], device="cuda")
+    low = (x + top.repeat((T + 11) // 12)[:T, None]).to(dtype)
+    spread = low.clone()
+    spread[:, 1:6] -= 40  # some of a token's experts in range, others below it
+    spread[:, 20] = -3.0
+    one_high = rand(T, 40, seed=1, dtype=dtype)
+    bias = torch.zeros(40, device="cuda")
+    bias[5:12] = 8.0  # chosen first, far below the largest logit
+    one_high[:, 5:12] -= 120
+    one_high[T // 2:, 5:12] -= 200
+    infinite = one_high.clone()
+    infinite[:, 5] = np.inf
+    for kw in (dict(), dict(scale=2.5), dict(renormalize=False, scale=3.0),
+               dict(n_group=4, topk_group=2, group_score="top2")):
+        for logits in (low, spread):
+            check_route(i4g, logits, 5, scoring="sigmoid", **kw)
+        check_route(i4g, one_high, 5, bias=bias, **kw)
+        check_route(i4g, infinite, 5, bias=bias, **kw)
+    w = i4g.route(low[:11], 5, scoring="sigmoid").weights.sum(1)
+    assert ((w - 1).abs() <= 8 * 2.0 ** -24).all()  # five roundings of the weights
+
+
 def test_route_all_rows_masked(i4g):
     for T in (4, 600):
         r = check_route(i4g, torch.full((T, 16), -np.inf, device="cuda"), 4)
