@@ -190,6 +190,18 @@ __device__ __forceinline__ bool choose(const Args& a, int lane, const float (&x)
     const bool whole_lanes = a.E == 32 * V && 32 % a.n_group == 0;
     const int span = 32 / a.n_group;  // lanes of a group, if it is whole lanes
     F mine = -INFINITY;               // lane g: group g's score
+    F largest = 0;                    // and the larger magnitude of its terms
+    // the two terms of a sum may cancel, so its error goes by them
+    const auto score_of = [&](K best, K second, F& size) {
+      F score = best ? value_of(best) : -INFINITY;
+      size = best ? fabs(score) : F(0);
+      if (a.top2 && second) {
+        const F next = value_of(second);
+        size = fmax(size, fabs(next));
+        score += next;
+      }
+      return score;
+    };
     if (whole_lanes) {
       // the best two of a group's lanes meet in a few exchanges
       K best = 0, second = 0;
@@ -203,9 +215,10 @@ __device__ __forceinline__ bool choose(const Args& a, int lane, const float (&x)
         second = max(max(second, os), min(best, ob));
         best = max(best, ob);
       }
-      F score = best ? value_of(best) : -INFINITY;
-      if (a.top2 && second) score += value_of(second);
+      F size_of;
+      const F score = score_of(best, second, size_of);
       mine = __shfl_sync(kAll, score, (lane * span) & 31);
+      if (tol > 0) largest = __shfl_sync(kAll, size_of, (lane * span) & 31);
     } else {
       // a group may start and end inside a lane: a pass over the warp for each
       for (int g = 0; g < a.n_group; ++g) {
@@ -218,13 +231,17 @@ __device__ __forceinline__ bool choose(const Args& a, int lane, const float (&x)
           best = max(best, k);
         }
         const K top = warp_max(best);
-        F score = top ? value_of(top) : -INFINITY;
+        K next = 0;
         if (a.top2) {
           const unsigned holders = __ballot_sync(kAll, best == top);
-          const K next = warp_max(lane == __ffs(holders) - 1 ? second : best);
-          if (next) score += value_of(next);
+          next = warp_max(lane == __ffs(holders) - 1 ? second : best);
         }
-        if (lane == g) mine = score;
+        F size_of;
+        const F score = score_of(top, next, size_of);
+        if (lane == g) {
+          mine = score;
+          largest = size_of;
+        }
       }
     }
     int rank = 0;
@@ -235,13 +252,15 @@ __device__ __forceinline__ bool choose(const Args& a, int lane, const float (&x)
     const bool kept = lane < a.n_group && rank < a.topk_group;
     const unsigned in = __ballot_sync(kAll, kept);
     if (tol > 0 && by_score && a.topk_group < a.n_group) {
-      // the last group in against the first one out
-      const unsigned at_in = __ballot_sync(kAll, lane < a.n_group && rank == a.topk_group - 1);
-      const unsigned at_out = __ballot_sync(kAll, lane < a.n_group && rank == a.topk_group);
-      const F lowest_in = __shfl_sync(kAll, mine, __ffs(at_in) - 1);
-      const F highest_out = __shfl_sync(kAll, mine, __ffs(at_out) - 1);
-      if (highest_out > -INFINITY)
-        sure = lowest_in - highest_out > 2 * tol * fmax(F(1), fabs(lowest_in));
+      // what each group's score can be: the least of those in against the most
+      // of those out (an infinite one is left to FP64; largest 0: no members)
+      const F error = tol * fmax(F(1), largest);
+      const bool finite = error < INFINITY && (fabs(mine) < INFINITY || largest == 0);
+      const F least = kept ? (finite ? mine - error : -INFINITY) : INFINITY;
+      const F most =
+          lane < a.n_group && !kept ? (finite ? mine + error : INFINITY) : -INFINITY;
+      const K lowest_in = ~warp_max(~key_of(least)), highest_out = warp_max(key_of(most));
+      sure = lowest_in > highest_out || highest_out == key_of(F(-INFINITY));
     }
     int g = whole_lanes ? lane / span : e0 / size;
     int next = whole_lanes ? a.E : (g + 1) * size;

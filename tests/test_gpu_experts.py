@@ -74,6 +74,29 @@ def test_route_ties_go_to_the_lowest_index(i4g):
     check_route(i4g, x * 1e-3, 8, scoring="sigmoid", bias=b)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,G", [(8, 2), (32, 4), (60, 6)])
+def test_route_groups_whose_terms_cancel(i4g, scoring, E, G):
+    """A group's two best may be large and of opposite sign: the order of their
+    sums is still FP64's. Biases that no FP32 score could resolve, masks by the
+    type's lowest value and infinite ones among them."""
+    x = rand(1000, E, seed=E, dtype=torch.float32)
+    bias = torch.full((E,), -2.0 ** 23, device="cuda")
+    size = E // G
+    for g in range(G):
+        bias[g * size], bias[g * size + 1] = 2.0 ** (20 - g % 2), -2.0 ** (20 - g % 2)
+    kw = dict(scoring=scoring, n_group=G, group_score="top2")
+    check_route(i4g, x, 2, bias=bias, topk_group=1, **kw)
+    check_route(i4g, x, 2, bias=-bias, topk_group=G - 1, **kw)
+    bias[size:] = torch.finfo(torch.float32).min
+    check_route(i4g, x, 2, bias=bias, topk_group=1, **kw)
+    bias[-size:] = -2.9e38  # sums that FP32 cannot hold, in order
+    check_route(i4g, x, 2, bias=bias, topk_group=min(2, G - 1), **kw)
+    bias[:size] = 0.0
+    bias[-1] = np.inf
+    check_route(i4g, x, 2, bias=bias, topk_group=1, **kw)
+
+
 def test_route_masks_infinities_and_nan(i4g):
     x = rand(300, 32, seed=4, dtype=torch.float32)
     x[5] = -np.inf          # a padded token
