@@ -449,7 +449,9 @@ __global__ void __launch_bounds__(Cfg<TILE_M>::THREADS, 1)
   #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int r = min((lane + 32 * q) * 4 + i, w.rows - 1);
-              src[q][i] = a.rows[w.row0 + r] / a.row_div;
+              // a negative row becomes -1: the division alone would round to row 0
+              const int pair = a.rows[w.row0 + r];
+              src[q][i] = (pair / a.row_div) | (pair >> 31);
             }
         }
         const int u0 = static_cast<int>(uniform(w.u0)), u1 = static_cast<int>(uniform(w.u1));

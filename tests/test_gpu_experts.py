@@ -349,6 +349,38 @@ def test_experts_bad_tables_are_clamped(i4g):
     assert i4g.device_status() == 0
 
 
+@pytest.mark.parametrize("T,E,k,K,N", [(9, 8, 2, 320, 384), (40, 12, 8, 128, 128),
+                                       (240, 8, 2, 1088, 4864), (1500, 5, 4, 576, 4864)])
+def test_experts_rows_outside_a_read_as_zeros(i4g, T, E, k, K, N):
+    """-1 (routing's own mark) down to -(k - 1), and rows behind A: zeros, whether
+    they are gathered inside the product or copied ahead of it."""
+    w = rand(E, K, N, seed=1, scale=0.05)
+    ex = i4g.QuantizedExperts.from_weight(w, 64)
+    r = routing_of(i4g, choices("random", T, E, k), E)
+    a = rand(T, K, seed=2)
+    bias = rand(E, N, seed=3)
+    rows = r.rows.clone()
+    outside = torch.arange(T * k, device="cuda") % 5 < 2
+    marks = torch.tensor([-1, 1 - k, T * k, -(2 ** 31), 2 ** 31 - 1], dtype=torch.int32,
+                         device="cuda")
+    rows[outside] = marks[torch.arange(int(outside.sum()), device="cuda") % 5]
+    expert = torch.bucketize(torch.arange(T * k, device="cuda"), r.offsets[1:].long(), right=True)
+    zeros = bias[expert].relu()
+    whole = ex(a, r, bias=bias, activation="relu")
+    need = i4g.experts_workspace_size(T * k, E, N, K)
+    for n in (0, need):
+        ws = torch.zeros(n, dtype=torch.uint8, device="cuda") if n else None
+        got = torch.empty(T * k, N, dtype=torch.float16, device="cuda")
+        i4g.launch_experts(a, T, ex.tiles, ex.scales, got, r.offsets, rows, k, T * k, E, N, K, 64,
+                           bias=bias, activation="relu", workspace=ws)
+        assert torch.equal(got[outside], zeros[outside])
+        # elsewhere what the rows inside A gave: two roundings to FP16, and sums of
+        # magnitudes up to 60 in another order, 2e-5 of them
+        near = (got - whole)[~outside].abs() <= 2.0 ** -9 * whole[~outside].abs() + 2.0 ** -9
+        assert near.all()
+    assert i4g.device_status() == 0
+
+
 def test_experts_offsets_that_fall_stay_in_the_workspace(i4g):
     """Offsets that fall and rise again name more tiles than any routing: nothing is
     written, neither to C nor behind the workspace (guards of 1 MB around both)."""
