@@ -99,7 +99,9 @@ class QuantizedExperts:
                      stream=None) -> "QuantizedExperts":
         """One weight per expert of the fp16 [E, K, F] gate and up projections, for
         calls with gated=True."""
-        return cls.from_weight(interleave_gate_up(gate, up), group, stream)
+        dev = cuda_device(gate, "gate")
+        with on(dev, stream, gate, up):  # the joined weights belong to the stream that reads them
+            return cls.from_weight(interleave_gate_up(gate, up), group)
 
     @classmethod
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, K: int, N: int, group: int,

@@ -40,12 +40,12 @@ class QuantizedLinear:
         layouts, in one pass."""
         if w.dtype != torch.float16 or w.dim() != 2 or not w.is_cuda:
             raise TypeError("weight must be a 2-D float16 CUDA tensor [K, N]")
-        w = w.contiguous()
         K, N = w.shape
         dev = w.device
-        tiles = torch.empty(K * N // 2, dtype=torch.uint8, device=dev)
-        rscales = torch.empty((K // group) * N, dtype=torch.float16, device=dev)
-        launch_quantize_repack(w, tiles, rscales, K, N, group, stream)
+        with on(dev, stream, w):
+            tiles = torch.empty(K * N // 2, dtype=torch.uint8, device=dev)
+            rscales = torch.empty((K // group) * N, dtype=torch.float16, device=dev)
+            launch_quantize_repack(w.contiguous(), tiles, rscales, K, N, group)
         return cls(tiles, rscales, K, N, group)
 
     @classmethod
@@ -53,17 +53,20 @@ class QuantizedLinear:
                      stream=None) -> "QuantizedLinear":
         """One weight of the fp16 [K, F] gate and up projections, for calls with
         gated=True (F % 64 == 0; a column's codes do not depend on its place)."""
-        return cls.from_weight(interleave_gate_up(gate, up), group, stream)
+        dev = cuda_device(gate, "gate")
+        with on(dev, stream, gate, up):  # the joined weight belongs to the stream that reads it
+            return cls.from_weight(interleave_gate_up(gate, up), group)
 
     @classmethod
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, K: int, N: int,
                     group: int, stream=None) -> "QuantizedLinear":
         """Repack reference-layout codes ([K][N] nibbles) and scales ([K/g][N])."""
-        dev = packed.device
-        tiles = torch.empty(K * N // 2, dtype=torch.uint8, device=dev)
-        rscales = torch.empty((K // group) * N, dtype=torch.float16, device=dev)
-        launch_repack_umma(packed, tiles, K, N, stream)
-        launch_repack_scales_128(scales, rscales, K, N, group, stream)
+        dev = cuda_device(packed, "packed")
+        with on(dev, stream, packed, scales):
+            tiles = torch.empty(K * N // 2, dtype=torch.uint8, device=dev)
+            rscales = torch.empty((K // group) * N, dtype=torch.float16, device=dev)
+            launch_repack_umma(packed, tiles, K, N)
+            launch_repack_scales_128(scales, rscales, K, N, group)
         return cls(tiles, rscales, K, N, group)
 
     def shard(self, world: int, rank: int) -> "QuantizedLinear":

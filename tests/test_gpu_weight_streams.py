@@ -1,0 +1,91 @@
+"""Weights made on an explicit stream while the current one is busy: every step
+of their making runs on the stream that was given, and what it allocates is that
+stream's."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def i4g():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    import sm_120__gemm_b200 as m
+    m.load()
+    return m
+
+
+def rand(*shape, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * 0.05).half()
+
+
+def while_busy(make, temporary):
+    """make(stream) with 50 ms of work ahead on the current stream, the memory a
+    temporary of that shape would get holding something else."""
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    for stream in (s, s.cuda_stream):
+        junk = torch.full(temporary, 3.0, dtype=torch.float16, device="cuda")
+        torch.cuda.synchronize()
+        del junk
+        torch.cuda._sleep(100_000_000)
+        made = make(stream)
+        # what the current stream frees and takes next must not be in use on s
+        torch.full(temporary, -3.0, dtype=torch.float16, device="cuda")
+        torch.cuda.synchronize()
+        yield made
+
+
+def same(a, b):
+    return torch.equal(a.tiles, b.tiles) and torch.equal(a.scales, b.scales)
+
+
+def test_linear_from_gate_up(i4g):
+    gate, up = rand(1024, 2048, seed=1), rand(1024, 2048, seed=2)
+    want = i4g.QuantizedLinear.from_gate_up(gate, up, 64)
+    for got in while_busy(lambda s: i4g.QuantizedLinear.from_gate_up(gate, up, 64, stream=s),
+                          (1024, 4096)):
+        assert same(got, want)
+
+
+def test_experts_from_gate_up(i4g):
+    gate, up = rand(3, 1024, 1024, seed=1), rand(3, 1024, 1024, seed=2)
+    want = i4g.QuantizedExperts.from_gate_up(gate, up, 64)
+    for got in while_busy(lambda s: i4g.QuantizedExperts.from_gate_up(gate, up, 64, stream=s),
+                          (3, 1024, 2048)):
+        assert same(got, want)
+
+
+def test_from_weight_with_strides(i4g):
+    w = rand(2048, 1024, seed=3).t()  # made contiguous inside the call
+    want = i4g.QuantizedLinear.from_weight(w, 128)
+    for got in while_busy(lambda s: i4g.QuantizedLinear.from_weight(w, 128, stream=s),
+                          (1024, 2048)):
+        assert same(got, want)
+    e = rand(2, 1024, 512, seed=4).transpose(1, 2)
+    want = i4g.QuantizedExperts.from_weight(e, 32)
+    for got in while_busy(lambda s: i4g.QuantizedExperts.from_weight(e, 32, stream=s),
+                          (1, 512, 1024)):
+        assert same(got, want)
+
+
+def test_from_packed(i4g):
+    K, N, g = 512, 1024, 64
+    packed = torch.randint(0, 256, (K * N // 2,), dtype=torch.uint8, device="cuda")
+    scales = rand(K // g, N, seed=5).abs()
+    want = i4g.QuantizedLinear.from_packed(packed, scales, K, N, g)
+    for got in while_busy(lambda s: i4g.QuantizedLinear.from_packed(packed, scales, K, N, g,
+                                                                    stream=s), (K, N // 4)):
+        assert same(got, want)
+
+
+def test_refuses_weights_on_the_cpu(i4g):
+    cpu = torch.zeros(64, 128, dtype=torch.float16)
+    for call in (lambda: i4g.QuantizedLinear.from_weight(cpu, 64),
+                 lambda: i4g.QuantizedLinear.from_gate_up(cpu, cpu, 64),
+                 lambda: i4g.QuantizedExperts.from_gate_up(cpu[None], cpu[None], 64)):
+        with pytest.raises(TypeError):
+            call()
