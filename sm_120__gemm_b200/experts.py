@@ -132,7 +132,7 @@ class QuantizedExperts:
         if kind is None:
             raise ValueError(f"unknown activation {activation!r}")
         dev = cuda_device(self.tiles, "the weights")
-        with on(dev, stream, a, routing.offsets, routing.rows, bias, out):
+        with on(dev, stream, self.tiles, self.scales, a, routing.offsets, routing.rows, bias, out):
             return binding().experts_gemm(a, self.tiles, self.scales, self.E, self.K, self.N,
                                           self.group, routing.offsets, routing.rows,
                                           routing.slots, gather, bias, kind, gated, out, fp32_out)

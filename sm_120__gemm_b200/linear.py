@@ -90,6 +90,9 @@ class QuantizedLinear:
             return self._epilogue(a, out, fp32_out, stream, bias, activation, gated, residual)
         if a.dtype != torch.float16 or a.dim() != 2 or a.shape[1] != self.K:
             raise ValueError(f"A must be float16 [M, {self.K}]")
+        if stream is not None:
+            with on(self.tiles.device, stream, self.tiles, self.scales, a, out):
+                return self(a, out, fp32_out)
         a = a.contiguous()
         M = a.shape[0]
         if out is None:
@@ -105,6 +108,6 @@ class QuantizedLinear:
         if kind is None:
             raise ValueError(f"unknown activation {activation!r}")
         dev = cuda_device(self.tiles, "the weight")
-        with on(dev, stream, a, bias, residual, out):
+        with on(dev, stream, self.tiles, self.scales, a, bias, residual, out):
             return binding().gemm_epilogue(a, self.tiles, self.scales, self.K, self.N, self.group,
                                            bias, kind, gated, residual, out, fp32_out)

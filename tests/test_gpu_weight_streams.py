@@ -82,6 +82,57 @@ def test_from_packed(i4g):
         assert same(got, want)
 
 
+@pytest.mark.parametrize("kind", ["plain", "fp32", "epilogue", "experts"])
+def test_weights_dropped_after_their_last_call(i4g, kind):
+    """A layer and its inputs may go right after a call on another stream: their
+    memory is not reused under the kernel."""
+    K, N, M = 1024, 2048, 24
+    a = rand(M, K, seed=1)
+    s = torch.cuda.Stream()
+
+    def layer():
+        if kind == "experts":
+            return i4g.QuantizedExperts.from_weight(rand(2, K, N, seed=2), 64)
+        return i4g.QuantizedLinear.from_weight(rand(K, N, seed=2), 64)
+
+    def call(m, x, **kw):
+        if kind == "experts":
+            r = i4g.route(torch.zeros(M, 2, device="cuda"), 1, **kw)
+            return m(x, r, activation="silu", **kw)
+        return m(x, fp32_out=(kind == "fp32"), activation="silu" if kind == "epilogue" else "none",
+                 **kw)
+
+    want = call(layer(), a)
+    torch.cuda.synchronize()
+    for stream in (s, s.cuda_stream):
+        m, x = layer(), a.clone()
+        sizes = [(t.numel(), t.dtype) for t in (m.tiles, m.scales, x)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(50_000_000)
+        got = call(m, x, stream=stream)
+        del m, x
+        taken = [torch.zeros(n, dtype=t, device="cuda") for n, t in sizes]
+        s.synchronize()
+        assert torch.equal(got, want)
+        del taken
+
+
+def test_strided_rows_on_a_stream(i4g):
+    """Rows that the call makes contiguous are copied on the stream that was given."""
+    lin = i4g.QuantizedLinear.from_weight(rand(256, 512, seed=2), 64)
+    x = rand(256, 40, seed=3)
+    want = lin(x.t())
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.full((40, 256), 3.0, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)
+    got = lin(x.t(), stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_refuses_weights_on_the_cpu(i4g):
     cpu = torch.zeros(64, 128, dtype=torch.float16)
     for call in (lambda: i4g.QuantizedLinear.from_weight(cpu, 64),
