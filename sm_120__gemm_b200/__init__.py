@@ -28,7 +28,7 @@ __all__ = [
     "launch_inverse_repack_umma", "launch_final", "launch_final_fp32", "launch_gemm_variant",
     "gemm_workspace_size", "launch_final_ws", "launch_final_fp32_ws", "workspace_for",
     "launch_final_to_peers", "ipc_handle", "ipc_open", "ipc_close", "peer_barrier",
-    "shard_range", "device_status", "selftest_wait_timeout", "plan", "set_decode_schedule",
+    "shard_range", "device_status", "reset_workspaces", "selftest_wait_timeout", "plan", "set_decode_schedule",
     "kernel_config", "kernel_resources", "max_pairs",
     "launch_final_epilogue", "gemm_epilogue_workspace_size", "launch_route",
     "route_workspace_size", "launch_experts", "experts_workspace_size", "launch_combine",
@@ -433,10 +433,31 @@ def shard_range(K: int, N: int, group: int, world: int, rank: int):
 
 
 def device_status(stream=None) -> int:
-    """Read and clear the device status word (0, or -8 after a wait timeout)."""
+    """Read and clear the device status word (0, or -8 after a wait timeout; then
+    the package's workspaces are reset, see ``reset_workspaces``)."""
     out = _i()
     _call("i4g_device_status", ctypes.byref(out), _stream(stream))
+    if out.value:
+        reset_workspaces()
     return out.value
+
+
+def reset_workspaces() -> None:
+    """Brings the workspaces the package holds back to zeroed arrival counters. A
+    launch that gave up on a wait leaves counters behind, and a later call would
+    take partial sums for whole ones. ``device_status`` calls it when it finds a
+    timeout; a caller that reads the status word otherwise calls it itself, as it
+    zeroes the workspaces it owns."""
+    import torch
+    from . import launching
+    if launching._binding is not None:
+        launching._binding.reset_workspaces()
+    # buffers of the plain product may be part of captured graphs: zeroed where
+    # they are, with nothing running on any stream
+    for ws in _workspaces.values():
+        torch.cuda.synchronize(ws.device)
+        ws[:4096].zero_()
+        torch.cuda.synchronize(ws.device)
 
 
 def selftest_wait_timeout(limit_ns: int, stream=None) -> None:

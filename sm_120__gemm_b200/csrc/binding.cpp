@@ -16,6 +16,7 @@
 #include <optional>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "../../include/i4g.h"
 
@@ -92,6 +93,29 @@ int narrow(int64_t v, const char* name) {
 // calls.
 constexpr int64_t kCounterBytes = 4096;
 
+struct Held {
+  std::mutex mutex;
+  std::map<std::pair<int, cudaStream_t>, Tensor> of;  // by device and stream
+};
+Held& held() {
+  static Held& h = *new Held;  // lives as long as the process
+  return h;
+}
+
+// A launch that gave up on a wait leaves counters behind: every buffer is
+// dropped (its memory stays its stream's), the next call makes a zeroed one.
+void reset_workspaces() {
+  std::lock_guard<std::mutex> lock(held().mutex);
+  held().of.clear();
+}
+
+std::vector<Tensor> workspaces() {
+  std::lock_guard<std::mutex> lock(held().mutex);
+  std::vector<Tensor> all;
+  for (const auto& entry : held().of) all.push_back(entry.second);
+  return all;
+}
+
 Tensor workspace(size_t need, at::Device device, cudaStream_t stream) {
   if (need == 0) return Tensor();
   const int64_t bytes = static_cast<int64_t>(need);
@@ -100,11 +124,8 @@ Tensor workspace(size_t need, at::Device device, cudaStream_t stream) {
     ws.narrow(0, 0, kCounterBytes).zero_();
     return ws;
   }
-  using Key = std::pair<int, cudaStream_t>;
-  static auto& held = *new std::map<Key, Tensor>;  // lives as long as the process
-  static std::mutex mutex;
-  std::lock_guard<std::mutex> lock(mutex);
-  Tensor& ws = held[Key(device.index(), stream)];
+  std::lock_guard<std::mutex> lock(held().mutex);
+  Tensor& ws = held().of[{device.index(), stream}];
   if (!ws.defined() || ws.numel() < bytes) {
     ws = empty({bytes}, at::kByte, device);
     ws.narrow(0, 0, kCounterBytes).zero_();
@@ -304,4 +325,6 @@ PYBIND11_MODULE(_binding, m) {
   m.def("experts_gemm", &experts_gemm);
   m.def("route", &route);
   m.def("combine", &combine);
+  m.def("reset_workspaces", &reset_workspaces);
+  m.def("workspaces", &workspaces);
 }

@@ -207,6 +207,34 @@ def test_workspace_none_small_and_enough_agree(i4g):
             assert int(ws[:4096].count_nonzero()) == 0, "arrival counters not reset"
 
 
+def test_counters_left_by_a_timeout_are_reset(i4g):
+    """What a launch that gave up leaves in the workspaces the package holds does
+    not reach later calls: the status call that reports it resets them."""
+    import sm_120__gemm_b200._binding as binding
+    lin, _ = make(i4g, 8192, 512, 64)
+    a, b = rand(24, 8192, seed=1), rand(600, 8192, seed=2)
+    assert i4g.gemm_epilogue_workspace_size(24, 512, 8192) > 0
+    assert i4g.gemm_workspace_size(600, 512, 8192) > 0
+    want, plain = lin(a, activation="silu"), lin(b)
+    s = torch.cuda.Stream()
+    lin(a, activation="silu", stream=s)
+    torch.cuda.synchronize()
+    buffers = binding.workspaces() + list(i4g._workspaces.values())
+    assert len(binding.workspaces()) >= 2 and i4g._workspaces
+    for ws in buffers:
+        ws[:4096].view(torch.int32).fill_(1)  # as half-arrived tiles leave them
+    i4g.selftest_wait_timeout(1000)
+    assert i4g.device_status() == -8
+    assert not binding.workspaces()
+    assert all(not ws[:4096].any() for ws in i4g._workspaces.values())
+    for _ in range(2):
+        assert torch.equal(lin(a, activation="silu"), want) and torch.equal(lin(b), plain)
+        got = lin(a, activation="silu", stream=s)
+        s.synchronize()
+        assert torch.equal(got, want)
+    assert i4g.device_status() == 0 and binding.workspaces()
+
+
 def test_graphs_share_nothing(i4g):
     """Two captured graphs replayed on two streams at once, and eager calls
     between: every result as if run alone."""
