@@ -291,12 +291,22 @@ int i4g_route(const void* logits, int fp32_logits, int ld_logits, const float* b
  * into expert order it also holds that copy (its counters are the first 4096
  * bytes either way). The size is for these arguments, and fewer pairs can ask
  * for more; a call with less than it asks for is slower, not wrong. pairs = 0
- * returns at once. */
+ * returns at once.
+ * The _parts forms take the two halves apart, for callers that keep a
+ * workspace: `kept` bytes of counters and partial sums (zeroed once, one per
+ * stream; 0: none) and `scratch` bytes for the row copy (0: none is made), which
+ * is one call's alone, needs no zeroing and is 256-byte aligned. */
 int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes);
 int i4g_experts_gemm(const void* A, int a_rows, const uint8_t* tiles, const void* scales, void* C,
                      const int32_t* offsets, const int32_t* rows, int row_div, int pairs, int E,
                      int N, int K, int group, const i4g_epilogue_t* epilogue, void* workspace,
                      size_t workspace_bytes, void* stream);
+int i4g_experts_workspace_parts(int pairs, int E, int N, int K, size_t* kept, size_t* scratch);
+int i4g_experts_gemm_parts(const void* A, int a_rows, const uint8_t* tiles, const void* scales,
+                           void* C, const int32_t* offsets, const int32_t* rows, int row_div,
+                           int pairs, int E, int N, int K, int group,
+                           const i4g_epilogue_t* epilogue, void* kept, size_t kept_bytes,
+                           void* scratch, size_t scratch_bytes, void* stream);
 
 /* out[t] = residual[t] + sum over places s of weights[t][s] * y[slots[t][s]]
  * (FP32, in the order of the places, then the residual, one rounding), y fp16

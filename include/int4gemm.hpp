@@ -154,6 +154,17 @@ inline void launch_experts(const half* a, int a_rows, const uint8_t* b, const ha
                "launch_experts");
 }
 
+// With a workspace kept per stream and a scratch of the call's own.
+inline void launch_experts(const half* a, int a_rows, const uint8_t* b, const half* s, void* c,
+                           const int32_t* offsets, const int32_t* rows, int row_div, int pairs,
+                           int E, int N, int K, int group, const i4g_epilogue_t& e, void* kept,
+                           size_t kept_bytes, void* scratch, size_t scratch_bytes,
+                           cudaStream_t stream) {
+  i4g_throw_if(i4g_experts_gemm_parts(a, a_rows, b, s, c, offsets, rows, row_div, pairs, E, N, K,
+                                      group, &e, kept, kept_bytes, scratch, scratch_bytes, stream),
+               "launch_experts");
+}
+
 inline void launch_combine(const half* y, int y_rows, const int32_t* slots, const float* weights,
                            const half* residual, half* out, int T, int top_k, int N,
                            cudaStream_t stream) {

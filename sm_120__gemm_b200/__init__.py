@@ -121,6 +121,9 @@ _SIGNATURES.update({
     "i4g_experts_workspace_size": [_i, _i, _i, _i, ctypes.POINTER(_sz)],
     "i4g_experts_gemm": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
                          ctypes.POINTER(Epilogue), _vp, _sz, _vp],
+    "i4g_experts_workspace_parts": [_i, _i, _i, _i, ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
+    "i4g_experts_gemm_parts": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
+                               ctypes.POINTER(Epilogue), _vp, _sz, _vp, _sz, _vp],
     "i4g_experts_combine": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
 })
 

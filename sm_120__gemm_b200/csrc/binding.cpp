@@ -226,19 +226,23 @@ Tensor experts_gemm(const Tensor& a_in, const Tensor& tiles, const Tensor& scale
     out = empty({pairs, cols}, dtype, on.device);
   }
   const int p = narrow(pairs, "T * top_k");
-  size_t need = 0;
-  check("i4g_experts_workspace_size",
-        i4g_experts_workspace_size(p, static_cast<int>(E), static_cast<int>(N),
-                                   static_cast<int>(K), &need));
+  size_t need = 0, copy = 0;
+  check("i4g_experts_workspace_parts",
+        i4g_experts_workspace_parts(p, static_cast<int>(E), static_cast<int>(N),
+                                    static_cast<int>(K), &need, &copy));
   const Tensor ws = workspace(need, on.device, on.stream);
-  check("i4g_experts_gemm",
-        i4g_experts_gemm(ptr(a), static_cast<int>(a_rows), tiles.const_data_ptr<uint8_t>(),
-                         ptr(scales), out.mutable_data_ptr(), offsets.const_data_ptr<int>(),
-                         gather ? rows.const_data_ptr<int>() : nullptr,
-                         static_cast<int>(top_k > 0 ? top_k : 1), p, static_cast<int>(E),
-                         static_cast<int>(N), static_cast<int>(K), static_cast<int>(group), &e,
-                         need ? ws.mutable_data_ptr() : nullptr,
-                         need ? static_cast<size_t>(ws.numel()) : 0, on.stream));
+  if (!gather) copy = 0;
+  Tensor scratch;  // the copied rows are this call's alone
+  if (copy) scratch = empty({static_cast<int64_t>(copy)}, at::kByte, on.device);
+  check("i4g_experts_gemm_parts",
+        i4g_experts_gemm_parts(ptr(a), static_cast<int>(a_rows), tiles.const_data_ptr<uint8_t>(),
+                               ptr(scales), out.mutable_data_ptr(), offsets.const_data_ptr<int>(),
+                               gather ? rows.const_data_ptr<int>() : nullptr,
+                               static_cast<int>(top_k > 0 ? top_k : 1), p, static_cast<int>(E),
+                               static_cast<int>(N), static_cast<int>(K), static_cast<int>(group),
+                               &e, need ? ws.mutable_data_ptr() : nullptr,
+                               need ? static_cast<size_t>(ws.numel()) : 0,
+                               copy ? scratch.mutable_data_ptr() : nullptr, copy, on.stream));
   return out;
 }
 

@@ -348,8 +348,9 @@ int check_epilogue(const i4g_epilogue_t& e, int N) {
 size_t rows_offset(size_t split_bytes) {
   return split_bytes > i4g::tc::kTicketBytes ? split_bytes : i4g::tc::kTicketBytes;
 }
+size_t row_copy_bytes(int pairs, int K) { return static_cast<size_t>(pairs) * K * 2; }
 size_t bytes_with_rows(size_t split_bytes, int pairs, int K) {
-  return rows_offset(split_bytes) + static_cast<size_t>(pairs) * K * 2;
+  return rows_offset(split_bytes) + row_copy_bytes(pairs, K);
 }
 
 // The checks and the launch that i4g_gemm_epilogue (offsets null) and
@@ -357,7 +358,7 @@ size_t bytes_with_rows(size_t split_bytes, int pairs, int K) {
 int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scales, void* C,
                const int* offsets, const int* rows, int row_div, int M, int E, int N, int K,
                int group, const i4g_epilogue_t* epilogue, void* workspace,
-               size_t workspace_bytes, void* stream) {
+               size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
   const i4g_epilogue_t plain{};
   const i4g_epilogue_t& e = epilogue ? *epilogue : plain;
   int st = check_group(K, group, true);
@@ -369,8 +370,8 @@ int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scal
     return fail(I4G_ERR_ALIGNMENT, "C must be aligned to its element size");
   if (!aligned(offsets, 4) || !aligned(rows, 4))
     return fail(I4G_ERR_ALIGNMENT, "offsets and rows must be 4-byte aligned");
-  if (workspace && !aligned(workspace, 256))
-    return fail(I4G_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  if (!aligned(workspace, 256) || !aligned(scratch, 256))
+    return fail(I4G_ERR_ALIGNMENT, "workspaces must be 256-byte aligned");
   DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != I4G_OK) return st;
   if (!offsets && i4g::epi::decode_is_faster(M, N, K, dev->sm_count)) {
@@ -387,13 +388,18 @@ int epi_common(const void* A, int a_rows, const uint8_t* tiles, const void* scal
   }
   const int tile_m = i4g::epi::choose_tile(M, E, N, K, dev->sm_count);
   const long tiles_most = i4g::epi::tiles_bound(tile_m, M, E, N);
-  // the workspace holds the split tail's part, then the activations in row
-  // order where they are copied; each is used if it fits
+  // the workspace holds the split tail's part, then, without a scratch of their
+  // own, the activations in row order where they are copied; each is used if it
+  // fits
   const size_t need = i4g::epi::workspace_bytes(tile_m, tiles_most, K, dev->sm_count);
   const bool split = workspace && need > 0 && workspace_bytes >= need;
-  if (rows && workspace && workspace_bytes >= bytes_with_rows(need, M, K) &&
+  if (!scratch && workspace && workspace_bytes >= bytes_with_rows(need, M, K)) {
+    scratch = static_cast<char*>(workspace) + rows_offset(need);
+    scratch_bytes = row_copy_bytes(M, K);
+  }
+  if (rows && scratch && scratch_bytes >= row_copy_bytes(M, K) &&
       i4g::epi::copy_rows_first(tile_m, M, E, N, K, dev->sm_count)) {
-    __half* copy = reinterpret_cast<__half*>(static_cast<char*>(workspace) + rows_offset(need));
+    __half* copy = static_cast<__half*>(scratch);
     const cudaError_t g = i4g::epi::gather_rows(static_cast<const __half*>(A), a_rows, offsets,
                                                 rows, row_div, copy, M, E, K, dev->sm_count,
                                                 static_cast<cudaStream_t>(stream));
@@ -798,22 +804,30 @@ int i4g_gemm_epilogue(const void* A, const uint8_t* tiles, const void* scales, v
   if (M == 0) return I4G_OK;
   if (!A || !tiles || !scales || !C) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
   return epi_common(A, M, tiles, scales, C, nullptr, nullptr, 1, M, 1, N, K, group, epilogue,
-                    workspace, workspace_bytes, stream);
+                    workspace, workspace_bytes, nullptr, 0, stream);
 }
 
 int i4g_experts_workspace_size(int pairs, int E, int N, int K, size_t* bytes) {
   if (!bytes) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
-  *bytes = 0;
+  size_t kept = 0, scratch = 0;
+  const int st = i4g_experts_workspace_parts(pairs, E, N, K, &kept, &scratch);
+  *bytes = scratch > 0 ? bytes_with_rows(kept, pairs, K) : kept;
+  return st;
+}
+
+int i4g_experts_workspace_parts(int pairs, int E, int N, int K, size_t* kept, size_t* scratch) {
+  if (!kept || !scratch) return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  *kept = *scratch = 0;
   int st = check_experts(pairs, E, N, K);
   if (st != I4G_OK) return st;
   if (pairs == 0) return I4G_OK;
   DeviceInfo* dev = nullptr;
   if ((st = current_device(&dev)) != I4G_OK) return st;
   const int tile_m = i4g::epi::choose_tile(pairs, E, N, K, dev->sm_count);
-  *bytes = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, pairs, E, N), K,
-                                     dev->sm_count);
+  *kept = i4g::epi::workspace_bytes(tile_m, i4g::epi::tiles_bound(tile_m, pairs, E, N), K,
+                                    dev->sm_count);
   if (i4g::epi::copy_rows_first(tile_m, pairs, E, N, K, dev->sm_count))
-    *bytes = bytes_with_rows(*bytes, pairs, K);
+    *scratch = row_copy_bytes(pairs, K);
   return I4G_OK;
 }
 
@@ -821,6 +835,16 @@ int i4g_experts_gemm(const void* A, int a_rows, const uint8_t* tiles, const void
                      const int32_t* offsets, const int32_t* rows, int row_div, int pairs, int E,
                      int N, int K, int group, const i4g_epilogue_t* epilogue, void* workspace,
                      size_t workspace_bytes, void* stream) {
+  return i4g_experts_gemm_parts(A, a_rows, tiles, scales, C, offsets, rows, row_div, pairs, E, N,
+                                K, group, epilogue, workspace, workspace_bytes, nullptr, 0,
+                                stream);
+}
+
+int i4g_experts_gemm_parts(const void* A, int a_rows, const uint8_t* tiles, const void* scales,
+                           void* C, const int32_t* offsets, const int32_t* rows, int row_div,
+                           int pairs, int E, int N, int K, int group,
+                           const i4g_epilogue_t* epilogue, void* kept, size_t kept_bytes,
+                           void* scratch, size_t scratch_bytes, void* stream) {
   const int st = check_experts(pairs, E, N, K);
   if (st != I4G_OK) return st;
   if (epilogue && epilogue->residual)
@@ -831,7 +855,7 @@ int i4g_experts_gemm(const void* A, int a_rows, const uint8_t* tiles, const void
   if (rows ? (a_rows < 1 || row_div < 1) : a_rows < pairs)
     return fail(I4G_ERR_SHAPE, "a_rows=%d row_div=%d for %d pairs", a_rows, row_div, pairs);
   return epi_common(A, a_rows, tiles, scales, C, offsets, rows, row_div, pairs, E, N, K, group,
-                    epilogue, workspace, workspace_bytes, stream);
+                    epilogue, kept, kept_bytes, scratch, scratch_bytes, stream);
 }
 
 static int check_route(int T, int E, int top_k) {

@@ -349,6 +349,39 @@ def test_experts_bad_tables_are_clamped(i4g):
     assert i4g.device_status() == 0
 
 
+def test_experts_row_copy_is_the_calls_own(i4g):
+    """Of a call's workspace only counters and partial sums stay with the package; the
+    copy of the gathered rows goes back when the call returns."""
+    T, E, k, K, N = 4096, 64, 8, 2048, 256
+    ex = i4g.QuantizedExperts.from_weight(rand(E, K, N, seed=1, scale=0.05), 64)
+    r = i4g.route(rand(T, E, seed=1, dtype=torch.float32), k)
+    a = rand(T, K, seed=2)
+    torch.cuda.synchronize()
+    i4g.reset_workspaces()
+    before = torch.cuda.memory_allocated()
+    y = ex(a, r)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated() - before - y.numel() * 2
+    copy = T * k * K * 2
+    assert i4g.experts_workspace_size(T * k, E, N, K) > copy  # rows are copied ahead here
+    assert held < copy // 2
+    # one buffer for everything gives the same, and so does a graph
+    ws = torch.zeros(i4g.experts_workspace_size(T * k, E, N, K), dtype=torch.uint8, device="cuda")
+    got = torch.empty_like(y)
+    i4g.launch_experts(a, T, ex.tiles, ex.scales, got, r.offsets, r.rows, k, T * k, E, N, K, 64,
+                       workspace=ws)
+    assert torch.equal(got, y)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ex(a, r)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        assert torch.equal(out, y)
+    assert torch.equal(ex(a.repeat_interleave(k, 0)[r.rows.long()], r, gather=False), y)
+    assert i4g.device_status() == 0
+
+
 @pytest.mark.parametrize("T,E,k,K,N", [(9, 8, 2, 320, 384), (40, 12, 8, 128, 128),
                                        (240, 8, 2, 1088, 4864), (1500, 5, 4, 576, 4864)])
 def test_experts_rows_outside_a_read_as_zeros(i4g, T, E, k, K, N):

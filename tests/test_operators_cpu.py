@@ -91,6 +91,22 @@ def test_experts_refusals(m, lib):
     assert experts(lib, pairs=0, a=None, c=None, offsets=None) == 0
 
 
+def test_experts_parts_refusals(m, lib):
+    def call(kept=None, scratch=None, E=4):
+        return lib.i4g_experts_gemm_parts(FAKE, 8, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 16, E, 128, 128,
+                                          64, None, kept, 0, scratch, 0, None)
+    assert call(E=0) == SHAPE
+    assert call(kept=vp(0x1080)) == ALIGN
+    assert call(scratch=vp(0x1010)) == ALIGN
+    kept, scratch = ctypes.c_size_t(), ctypes.c_size_t()
+    parts = lib.i4g_experts_workspace_parts
+    assert parts(16, 4, 128, 128, None, ctypes.byref(scratch)) == NULL
+    assert parts(16, 4, 128, 128, ctypes.byref(kept), None) == NULL
+    assert parts(16, 0, 128, 128, ctypes.byref(kept), ctypes.byref(scratch)) == SHAPE
+    assert parts(0, 4, 128, 128, ctypes.byref(kept), ctypes.byref(scratch)) == 0
+    assert kept.value == scratch.value == 0
+
+
 def route(m, lib, T=4, E=16, k=2, logits=FAKE, ld=16, out=FAKE, bias=None, offsets=FAKE, **opt):
     o = m.RouteOptions(0, 1, 1, 0, 1, 1.0)
     for name, v in opt.items():
