@@ -147,6 +147,7 @@ Tensor gemm_epilogue(const Tensor& a_in, const Tensor& tiles, const Tensor& scal
                      bool gated, const OptTensor& residual_in, const OptTensor& out_in,
                      bool fp32_out) {
   const Launch on(tiles);
+  want(scales, "scales", at::kHalf, on.device);
   want(a_in, "A", at::kHalf, on.device);
   if (a_in.dim() != 2 || a_in.size(1) != K)
     bad_value("A must be float16 [M, " + std::to_string(K) + "]");
@@ -197,6 +198,7 @@ Tensor experts_gemm(const Tensor& a_in, const Tensor& tiles, const Tensor& scale
                     const OptTensor& bias_in, int64_t activation, bool gated,
                     const OptTensor& out_in, bool fp32_out) {
   const Launch on(tiles);
+  want(scales, "scales", at::kHalf, on.device);
   want(a_in, "A", at::kHalf, on.device);
   if (slots.dim() != 2) bad_value("routing.slots must be [T, top_k]");
   const int64_t T = slots.size(0), top_k = slots.size(1), pairs = T * top_k;

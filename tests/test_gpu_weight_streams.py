@@ -133,6 +133,19 @@ def test_strided_rows_on_a_stream(i4g):
     assert torch.equal(got, want)
 
 
+def test_refuses_scales_elsewhere(i4g):
+    """Codes and scales live on one device: the call says so before it launches."""
+    lin = i4g.QuantizedLinear.from_weight(rand(64, 128), 64)
+    ex = i4g.QuantizedExperts.from_weight(rand(2, 64, 128), 64)
+    a = rand(4, 64)
+    r = i4g.route(torch.zeros(4, 2, device="cuda"), 1)
+    apart = i4g.QuantizedLinear(lin.tiles, lin.scales.cpu(), 64, 128, 64)
+    with pytest.raises(TypeError):
+        apart(a, activation="silu")
+    with pytest.raises(TypeError):
+        i4g.QuantizedExperts(ex.tiles, ex.scales.cpu(), 2, 64, 128, 64)(a, r)
+
+
 def test_refuses_weights_on_the_cpu(i4g):
     cpu = torch.zeros(64, 128, dtype=torch.float16)
     for call in (lambda: i4g.QuantizedLinear.from_weight(cpu, 64),
