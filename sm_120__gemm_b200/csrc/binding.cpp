@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/types.h>
+#include <torch/version.h>
 
 #include <map>
 #include <mutex>
@@ -327,6 +328,7 @@ Tensor combine(const Tensor& y_in, const Tensor& slots, const Tensor& weights,
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
+  m.attr("torch_version") = std::string(TORCH_VERSION);
   m.def("gemm_epilogue", &gemm_epilogue);
   m.def("experts_gemm", &experts_gemm);
   m.def("route", &route);
