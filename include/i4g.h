@@ -381,6 +381,19 @@ int i4g_plan(int M, int N, int K, int group, int fp32_out, int sm_count,
              size_t workspace_bytes, int* kernel, int* schedule, int* param,
              size_t* bytes);
 
+/* What i4g_gemm_epilogue (E = 0, M rows) or i4g_experts_gemm (M sorted rows over
+ * E >= 1 experts) would run on a device with sm_count SMs and the workspace it
+ * asks for, answered on the host:
+ *   *tile_rows:  activation rows a tile (16, 32, 64, 128, 256), or 0: the
+ *                decode kernel
+ *   *copy_rows:  1: gathered rows are copied into expert order first
+ *   *tail_tiles: tiles of the last, partial wave that are cut along K, into
+ *   *shares      equal runs of 64-k blocks (both 0: whole tiles)
+ * The experts' tail follows from the routing: expert_rows (host memory, [E])
+ * holds each expert's rows; NULL reports no tail for them. */
+int i4g_epilogue_plan(int M, int E, const int32_t* expert_rows, int N, int K, int sm_count,
+                      int* tile_rows, int* copy_rows, int* tail_tiles, int* shares);
+
 /* With the I4G_PAIR=1 environment variable (read at the first launch) the
  * tcgen05 kernel runs 256-row tiles on CTA pairs (thread-block clusters of
  * two, one 2-SM tensor-core instruction per pair, both operands from

@@ -28,7 +28,8 @@ __all__ = [
     "launch_inverse_repack_umma", "launch_final", "launch_final_fp32", "launch_gemm_variant",
     "gemm_workspace_size", "launch_final_ws", "launch_final_fp32_ws", "workspace_for",
     "launch_final_to_peers", "ipc_handle", "ipc_open", "ipc_close", "peer_barrier",
-    "shard_range", "device_status", "reset_workspaces", "selftest_wait_timeout", "plan", "set_decode_schedule",
+    "shard_range", "device_status", "reset_workspaces", "selftest_wait_timeout", "plan",
+    "epilogue_plan", "set_decode_schedule",
     "kernel_config", "kernel_resources", "max_pairs",
     "launch_final_epilogue", "gemm_epilogue_workspace_size", "launch_route",
     "route_workspace_size", "launch_experts", "experts_workspace_size", "launch_combine",
@@ -110,6 +111,8 @@ class RouteOptions(ctypes.Structure):
                 ("renormalize", _i), ("scale", ctypes.c_float)]
 
 
+_SIGNATURES["i4g_epilogue_plan"] = [_i, _i, ctypes.POINTER(ctypes.c_int32), _i, _i, _i,
+                                    *[ctypes.POINTER(_i)] * 4]
 _sz = ctypes.c_size_t
 _SIGNATURES.update({
     "i4g_gemm_epilogue_workspace_size": [_i, _i, _i, ctypes.POINTER(_sz)],
@@ -490,6 +493,19 @@ def plan(M: int, N: int, K: int, group: int, sm_count: int, workspace_bytes: int
           ctypes.byref(s), ctypes.byref(p), ctypes.byref(b))
     return {"kernel": PLAN_KERNELS[k.value], "schedule": PLAN_SCHEDULES[s.value],
             "param": p.value, "workspace_bytes": b.value}
+
+
+def epilogue_plan(M: int, N: int, K: int, sm_count: int, E: int = 0, expert_rows=None) -> dict:
+    """C ABI i4g_epilogue_plan: the tile height (0: decode kernel), row copy and split
+    tail of the epilogue product of M rows, or of M sorted rows over E experts
+    (expert_rows: how many each has), on a device with `sm_count` SMs (no device
+    needed)."""
+    if expert_rows is not None:
+        expert_rows = (ctypes.c_int32 * len(expert_rows))(*expert_rows)
+        E = len(expert_rows)
+    v = [_i() for _ in range(4)]
+    _call("i4g_epilogue_plan", M, E, expert_rows, N, K, sm_count, *map(ctypes.byref, v))
+    return dict(zip(("tile_rows", "copy_rows", "tail_tiles", "shares"), (x.value for x in v)))
 
 
 def kernel_config(variant: int, rows: int, group: int) -> dict:

@@ -1072,6 +1072,39 @@ int i4g_plan(int M, int N, int K, int group, int fp32_out, int sm_count,
   return I4G_OK;
 }
 
+int i4g_epilogue_plan(int M, int E, const int32_t* expert_rows, int N, int K, int sm_count,
+                      int* tile_rows, int* copy_rows, int* tail_tiles, int* shares) {
+  if (!tile_rows || !copy_rows || !tail_tiles || !shares)
+    return fail(I4G_ERR_NULL_POINTER, "null pointer argument");
+  *tile_rows = *copy_rows = *tail_tiles = *shares = 0;
+  const int weights = E == 0 ? 1 : E;
+  const int st = check_experts(M, weights, N, K);
+  if (st != I4G_OK) return st;
+  if (M < 1) return fail(I4G_ERR_SHAPE, "a plan needs rows");
+  if (sm_count < 1 || sm_count > 4096) return fail(I4G_ERR_SHAPE, "sm_count %d", sm_count);
+  // the same choices as epi_common
+  if (E == 0 && i4g::epi::decode_is_faster(M, N, K, sm_count)) return I4G_OK;
+  const int tile_m = i4g::epi::choose_tile(M, weights, N, K, sm_count);
+  *tile_rows = tile_m;
+  *copy_rows = E > 0 && i4g::epi::copy_rows_first(tile_m, M, E, N, K, sm_count);
+  const long most = i4g::epi::tiles_bound(tile_m, M, weights, N);
+  long tiles = most;
+  if (E > 0) {
+    if (!expert_rows) return I4G_OK;
+    long long all = 0;
+    tiles = 0;
+    for (int e = 0; e < E; ++e) {
+      if (expert_rows[e] < 0 || (all += expert_rows[e]) > M)
+        return fail(I4G_ERR_SHAPE, "the experts' rows are more than the %d there are", M);
+      tiles += (static_cast<long>(expert_rows[e]) + tile_m - 1) / tile_m * (N / 128);
+    }
+  }
+  const i4g::epi::Sched s = i4g::epi::schedule(tile_m, tiles, most, K, sm_count);
+  *tail_tiles = s.tail_tiles;
+  *shares = s.chunks;
+  return I4G_OK;
+}
+
 static int kernel_instance(int variant, int rows, int group) {
   int st = check_group(group, group, false);
   if (st != I4G_OK) return st;

@@ -229,6 +229,16 @@ int grid_for(int tile_m, long tiles, int K, int sm_count, bool split) {
   return static_cast<int>(std::max<long>(1, std::min<long>(most, sm_count)));
 }
 
+Sched schedule(int tile_m, long tiles, long tiles_most, int K, int sm_count) {
+  const bool split = workspace_bytes(tile_m, tiles_most, K, sm_count) > 0;
+  const int grid = grid_for(tile_m, tiles_most, K, sm_count, split);
+  const int bs = box_blocks(tile_m), kunits = (K / BK + bs - 1) / bs;
+  const int overhead = tile_m == 256   ? split_overhead_blocks<256>()
+                       : tile_m >= 64  ? split_overhead_blocks<64>()
+                                       : split_overhead_blocks<16>();
+  return make_sched(static_cast<int>(tiles), kunits, bs, grid, split, overhead);
+}
+
 cudaError_t launch(const CUtensorMap& act_map, int tile_m, bool gated, int group, const Args& args,
                    int grid, cudaStream_t stream) {
   switch (tile_m) {

@@ -56,6 +56,9 @@ long tiles_bound(int tile_m, int M, int E, int N);
 // Workspace of the split tail for any number of tiles (0: nothing to split).
 size_t workspace_bytes(int tile_m, long tiles, int K, int sm_count);
 int grid_for(int tile_m, long tiles, int K, int sm_count, bool split);
+// The schedule a launch of `tiles` tiles finds when its grid and workspace are
+// for `tiles_most`.
+Sched schedule(int tile_m, long tiles, long tiles_most, int K, int sm_count);
 cudaError_t launch(const CUtensorMap& act_map, int tile_m, bool gated, int group, const Args& args,
                    int grid, cudaStream_t stream);
 // The instances of one tile height (one translation unit each).
