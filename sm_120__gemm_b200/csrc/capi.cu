@@ -9,6 +9,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -443,6 +444,8 @@ int check_experts(int pairs, int E, int N, int K) {
   if (E < 1 || E > i4g::epi::kMaxExperts)
     return fail(I4G_ERR_SHAPE, "between 1 and %d experts (got %d)", i4g::epi::kMaxExperts, E);
   if (pairs < 0) return fail(I4G_ERR_SHAPE, "pairs %d is negative", pairs);
+  // a row index past the last tile still fits 32 bits
+  if (pairs > INT_MAX - 256) return fail(I4G_ERR_SHAPE, "%d rows are too many", pairs);
   const int st = check_shape(pairs > 0 ? pairs : 1, N, K);
   if (st != I4G_OK) return st;
   // tile indices are 32 bits

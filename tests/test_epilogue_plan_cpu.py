@@ -7,7 +7,7 @@ import pytest
 
 import tile_cases
 
-NULL = -1
+NULL, SHAPE = -1, -2
 HEIGHTS = {16, 32, 64, 128, 256}
 
 
@@ -61,6 +61,22 @@ def test_decode_kernel_and_whole_waves(m):
     assert m.epilogue_plan(1, 4096, 4096, 148, E=1)["tile_rows"] != 0  # experts: never decode
     assert m.epilogue_plan(17, 18944, 8192, 148)["shares"] == 0  # 148 tiles: no tail
     assert m.epilogue_plan(40, 4096, 64, 148)["shares"] == 0     # too short to cut
+
+
+def test_rows_up_to_32_bits(m):
+    """Row counts that a tile's height more would take past 32 bits are refused by every
+    entry point that takes them; the largest others have a plan."""
+    most = 2 ** 31 - 1 - 256
+    n = ctypes.c_size_t()
+    for E in (0, 1, 3):
+        assert m.epilogue_plan(most, 128, 64, 148, E=E)["tile_rows"] == 256
+        for rows in (most + 1, 2 ** 31 - 1):
+            with pytest.raises(m.I4GError):
+                m.epilogue_plan(rows, 128, 64, 148, E=E)
+    for rows in (most + 1, 2 ** 31 - 1):
+        lib = m.load()
+        assert lib.i4g_gemm_epilogue_workspace_size(rows, 128, 64, ctypes.byref(n)) == SHAPE
+        assert lib.i4g_experts_workspace_size(rows, 3, 128, 64, ctypes.byref(n)) == SHAPE
 
 
 def test_rows_of_experts_beyond_the_pairs(m):
