@@ -21,7 +21,7 @@ def binding():
         if not os.path.exists(os.path.join(HERE, "_binding.so")):
             raise ImportError(f"{HERE}/_binding.so is not built; run `make -C {HERE} python`")
         from . import _binding as module
-        if module.torch_version != torch.__version__.split("+")[0]:
+        if not torch.__version__.startswith(module.torch_version):
             raise ImportError(f"_binding.so was built against torch {module.torch_version}, not "
                               f"{torch.__version__}; run `make -C {HERE} python`")
         _binding = module

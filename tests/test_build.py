@@ -56,5 +56,22 @@ def test_python_part_follows_torch(tmp_path):
 
 def test_binding_names_the_torch_it_was_built_against():
     import torch
-    from sm_120__gemm_b200.launching import binding
-    assert binding().torch_version == torch.__version__.split("+")[0]
+    from sm_120__gemm_b200 import launching
+    module = launching.binding()
+    assert torch.__version__.startswith(module.torch_version) and module.torch_version
+
+
+def test_binding_of_another_torch_is_refused(monkeypatch):
+    import torch
+    from sm_120__gemm_b200 import launching
+    module = launching.binding()
+    for version, fits in (("2.11.0+cu128", True), ("2.11.0.dev20260101", True),
+                          ("2.12.0+cu128", False)):
+        monkeypatch.setattr(module, "torch_version", "2.11.0")
+        monkeypatch.setattr(torch, "__version__", version)
+        monkeypatch.setattr(launching, "_binding", None)
+        if fits:
+            launching.binding()
+        else:
+            with pytest.raises(ImportError):
+                launching.binding()
