@@ -18,7 +18,10 @@
 // and redone in FP64 (for that token alone) when two neighbours in the order,
 // or the last group in and the first group out, are closer than the FP32
 // error. Few tokens need it, so the choice costs FP32 and is the one the
-// definition gives in FP64.
+// definition gives in FP64. The weights of a token with a chosen score below
+// FP32's normal numbers are FP64's too. The FP64 parts are inlined and set the
+// kernels' 46 to 64 registers; above 256 experts, 16 experts a lane, they spill
+// (288 to 608 bytes of stores).
 //
 // One warp per token. Lane l holds experts l V .. l V + V - 1 (V = E / 32
 // rounded up), so among equal scores the lowest lane, and in it the lowest

@@ -41,7 +41,8 @@ def run(i4g, M, N, K, group, act="none", gated=False, bias=False, residual=False
     ref.check(got, *ref.linear(a, w64, act, gated, b, r, fp32))
 
 
-# every tile height, ragged and full
+# row counts around every tile height; at this size they run the decode kernel
+# and 16-row tiles (test_gpu_tile_heights.py asserts the height it runs)
 @pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 33, 64, 65, 100, 128, 129, 255, 257, 700])
 @pytest.mark.parametrize("gated", [False, True])
 def test_rows(i4g, M, gated):
@@ -74,8 +75,9 @@ def test_tile_heights(i4g, M, N, K, gated, fp32):
     run(i4g, M, N, K, 64, "gelu" if gated else "none", gated, bias=True, residual=True, fp32=fp32)
 
 
-# tails cut along K: few tiles and long K, more tiles than SMs, promotion; up to
-# 16 rows both kernels that serve them
+# few tiles and long K, more tiles than SMs, promotion; up to 16 rows both kernels
+# that serve them. Tails are cut along K at 16, 32 and 64 rows here, the last two run
+# whole 128-row tiles (test_gpu_tile_heights.py cuts at every height)
 @pytest.mark.parametrize("M,N,K", [(1, 128, 14336), (7, 256, 8192), (1, 28672, 2048),
                                    (3, 28672, 8192), (13, 20480, 4160), (16, 57344, 1024),
                                    (40, 4096, 8192), (64, 128, 6144 + 64), (100, 640, 8192),
