@@ -320,7 +320,11 @@ def workspace_for(M: int, N: int, K: int, device=None, stream=None):
     key = (dev.index, _stream(stream))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < need:
-        ws = torch.zeros(need, dtype=torch.uint8, device=dev)
+        from .launching import on
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        with on(dev, stream):  # zeroed on the stream that uses it
+            ws = torch.zeros(need, dtype=torch.uint8, device=dev)
         _workspaces[key] = ws
     return ws
 

@@ -133,6 +133,28 @@ def test_strided_rows_on_a_stream(i4g):
     assert torch.equal(got, want)
 
 
+def test_workspace_is_zeroed_on_its_stream(i4g):
+    M, N, K = 600, 512, 8192
+    need = i4g.gemm_workspace_size(M, N, K)
+    assert need > 4096
+    s = torch.cuda.Stream()
+    for stream in (s, s.cuda_stream):
+        i4g._workspaces.pop((torch.cuda.current_device(), s.cuda_stream), None)
+        torch.cuda.empty_cache()
+        junk = torch.full((need,), 3, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        del junk
+        torch.cuda._sleep(50_000_000)
+        ws = i4g.workspace_for(M, N, K, stream=stream)
+        with torch.cuda.stream(s):
+            seen = ws[:4096].clone()
+        s.synchronize()
+        assert not seen.any()
+        torch.cuda.synchronize()
+    i4g._workspaces.pop((None, s.cuda_stream), None)
+    assert i4g.workspace_for(M, N, K, device="cuda", stream=s).device == ws.device
+
+
 def test_refuses_scales_elsewhere(i4g):
     """Codes and scales live on one device: the call says so before it launches."""
     lin = i4g.QuantizedLinear.from_weight(rand(64, 128), 64)
