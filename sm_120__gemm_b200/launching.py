@@ -3,6 +3,7 @@ runs on, and the module that checks its tensors and makes the call."""
 from __future__ import annotations
 
 import contextlib
+import functools
 import os
 
 import torch
@@ -43,11 +44,21 @@ def on(device, stream, *used):
         if device.index == torch.cuda.current_device():
             return _current
         return torch.cuda.device(device)
+    return torch.cuda.stream(mark(device, stream, *used))
+
+
+@functools.lru_cache(maxsize=64)
+def _external(handle: int, device) -> torch.cuda.Stream:
+    return torch.cuda.ExternalStream(handle, device=device)
+
+
+def mark(device, stream, *used) -> torch.cuda.Stream:
+    """Marks the tensors in `used` as used on the explicit `stream`, which it returns."""
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
+        stream = _external(stream, device)
     elif stream.device != device:
         raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
     for t in used:
         if isinstance(t, torch.Tensor) and t.is_cuda:
             t.record_stream(stream)
-    return torch.cuda.stream(stream)
+    return stream

@@ -11,7 +11,7 @@ import torch
 
 from . import (ACTIVATIONS, launch_final_fp32_ws, launch_final_ws, launch_quantize_repack,
                launch_repack_scales_128, launch_repack_umma, shard_range, workspace_for)
-from .launching import binding, cuda_device, on
+from .launching import binding, cuda_device, mark, on
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -90,14 +90,18 @@ class QuantizedLinear:
             return self._epilogue(a, out, fp32_out, stream, bias, activation, gated, residual)
         if a.dtype != torch.float16 or a.dim() != 2 or a.shape[1] != self.K:
             raise ValueError(f"A must be float16 [M, {self.K}]")
-        if stream is not None:
-            with on(self.tiles.device, stream, self.tiles, self.scales, a, out):
-                return self(a, out, fp32_out)
-        a = a.contiguous()
         M = a.shape[0]
-        if out is None:
-            out = torch.empty(M, self.N, dtype=torch.float32 if fp32_out else torch.float16,
-                              device=a.device)
+        dtype = torch.float32 if fp32_out else torch.float16
+        if stream is not None:
+            s = mark(self.tiles.device, stream, self.tiles, self.scales, a, out)
+            if out is None or not a.is_contiguous():  # made on the stream, and its own
+                with torch.cuda.stream(s):
+                    a = a.contiguous()
+                    out = torch.empty(M, self.N, dtype=dtype, device=a.device) if out is None else out
+        else:
+            a = a.contiguous()
+            if out is None:
+                out = torch.empty(M, self.N, dtype=dtype, device=a.device)
         ws = workspace_for(M, self.N, self.K, a.device, stream)
         fn = launch_final_fp32_ws if fp32_out else launch_final_ws
         fn(a, self.tiles, self.scales, out, M, self.N, self.K, self.group, ws, stream)
